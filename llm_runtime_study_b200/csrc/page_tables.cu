@@ -1,0 +1,128 @@
+// The requests' page tables on the device, and a step's maps built from them.
+//
+// Every request slot has a row of a table [slots, width]: the ids of its pages, in the order of its tokens.  The host sends
+// only the cells that changed (pages taken since the last step); a step's block table, positions and slot map are made here
+// from the requests' lengths:
+//
+//   start_r        = max(kv_len_r - count_r, 0)
+//   q_start_r      = sum of counts of the entries before r
+//   positions_n    = start_e + (n - q_start_e)                    for the tokens n of entry e
+//   block_table_rc = tables[slots_r][c]  if c page_size < kv_len_r, else -1
+//   slot_map_n     = block_table[e][p / page_size] page_size + p % page_size, or -1 where there is no page
+//
+// Nothing but copies of a few bytes per token and column: what bounds it is the launch.
+#include "common.cuh"
+
+namespace b200 {
+
+// tables[rows[i]][columns[i]] = pages[i].  A cell outside the table is left alone.
+__global__ void page_table_set_kernel(int* __restrict__ tables, int table_rows, int width, const int* __restrict__ rows,
+                                      const int* __restrict__ columns, const int* __restrict__ pages, int n) {
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int row = rows[i], column = columns[i];
+  if (row < 0 || row >= table_rows || column < 0 || column >= width) return;
+  tables[static_cast<size_t>(row) * width + column] = pages[i];
+}
+
+struct StepMapsArgs {
+  const int* tables;
+  const int* slots;
+  const int* kv_len;
+  const int* counts;
+  int* block_table;
+  int* q_start;        // the rest may be null: not wanted
+  int* positions;
+  int* token_entry;
+  long long* slot_map;
+  int table_rows, width, out_width, entries, page_size, num_tokens;
+};
+
+constexpr int kMapThreads = 256;
+constexpr int kMapShare = 4 * kMapThreads;     // columns, and tokens, of an entry that one CTA takes at a time
+
+// One CTA per (entry, share of its columns and tokens).  The tokens before an entry are counted by every CTA itself (a step
+// has at most some hundred entries), so no CTA waits for another.  VEC: four columns to a 16-byte access.
+template <bool VEC>
+__global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const __grid_constant__ StepMapsArgs a) {
+  __shared__ int warp_sums[kMapThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, t = threadIdx.x;
+  const int slot = a.slots[r];
+  const bool known = slot >= 0 && slot < a.table_rows;
+  const int* row = a.tables + static_cast<size_t>(known ? slot : 0) * a.width;
+  const int length = max(a.kv_len[r], 0), page_size = a.page_size;
+  const int held = known && length > 0 ? min((length - 1) / page_size + 1, a.width) : 0;      // columns that hold a page
+  int* out = a.block_table + static_cast<size_t>(r) * a.out_width;
+  for (int c = (blockIdx.y * kMapThreads + t) * 4; c < a.out_width; c += gridDim.y * kMapShare) {
+    if (VEC) {
+      int4 v = c < held ? *reinterpret_cast<const int4*>(row + c) : make_int4(-1, -1, -1, -1);
+      if (c + 1 >= held) v.y = -1;
+      if (c + 2 >= held) v.z = -1;
+      if (c + 3 >= held) v.w = -1;
+      *reinterpret_cast<int4*>(out + c) = v;
+    } else {
+      for (int i = c; i < min(c + 4, a.out_width); ++i) out[i] = i < held ? row[i] : -1;
+    }
+  }
+  if (a.q_start == nullptr && a.positions == nullptr && a.token_entry == nullptr && a.slot_map == nullptr) return;
+  int before = 0;
+  for (int i = t; i < r; i += kMapThreads) before += max(a.counts[i], 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if ((t & 31) == 0) warp_sums[t >> 5] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < kMapThreads / 32; ++w) before += warp_sums[w];
+  const int count = max(a.counts[r], 0), start = max(length - count, 0);
+  if (a.q_start != nullptr && blockIdx.y == 0 && t == 0) {
+    a.q_start[r] = before;
+    if (r == a.entries - 1) a.q_start[r + 1] = before + count;
+  }
+  for (int i = blockIdx.y * kMapThreads + t; i < count; i += gridDim.y * kMapThreads) {
+    const int n = before + i;
+    if (static_cast<unsigned>(n) >= static_cast<unsigned>(a.num_tokens)) break;
+    const int position = start + i, column = position / page_size;
+    if (a.positions != nullptr) a.positions[n] = position;
+    if (a.token_entry != nullptr) a.token_entry[n] = r;
+    if (a.slot_map != nullptr) {
+      const int page = column < held ? row[column] : -1;
+      a.slot_map[n] = page < 0 ? -1 : static_cast<long long>(page) * page_size + (position - column * page_size);
+    }
+  }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_page_table_set(int* tables, int table_rows, int width, const int* rows, const int* columns, const int* pages,
+                                   int n, cudaStream_t stream) {
+  if (n <= 0) return 0;
+  if (table_rows <= 0 || width <= 0) return B200_ERR_BAD_SIZE;
+  const int threads = 128;
+  launch(page_table_set_kernel, dim3((n + threads - 1) / threads), dim3(threads), 0, stream, tables, table_rows, width, rows, columns,
+         pages, n);
+  return launch_status();
+}
+
+extern "C" int b200_step_maps(const int* tables, int table_rows, int width, const int* slots, const int* kv_len, const int* counts,
+                              int* block_table, int out_width, int* q_start, int* positions, int* token_entry, long long* slot_map,
+                              int entries, int page_size, int num_tokens, cudaStream_t stream) {
+  if (entries <= 0) return 0;
+  if (table_rows <= 0 || width <= 0 || out_width <= 0 || page_size <= 0 || num_tokens < 0) return B200_ERR_BAD_SIZE;
+  StepMapsArgs a{tables, slots, kv_len, counts, block_table, q_start, positions, token_entry, slot_map,
+                 table_rows, width, out_width, entries, page_size, num_tokens};
+  const bool vec = width % 4 == 0 && out_width % 4 == 0 && reinterpret_cast<uintptr_t>(tables) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(block_table) % 16 == 0;
+  // as many shares as the wider of a row's columns and a mean entry's tokens asks for
+  const int tokens = (num_tokens + entries - 1) / entries;
+  int shares = ((out_width > tokens ? out_width : tokens) + kMapShare - 1) / kMapShare;
+  if (shares > 64) shares = 64;
+  launch(vec ? step_maps_kernel<true> : step_maps_kernel<false>, dim3(entries, shares), dim3(kMapThreads), 0, stream, a);
+  return launch_status();
+}

@@ -362,6 +362,17 @@ def require(t: torch.Tensor, name: str, *, dtype=None, shape=None, dims=None) ->
     return t
 
 
+def require_here(t: torch.Tensor, name: str, align: int = 4) -> None:
+    """The tensor lies on the current CUDA device, whose stream the kernels go to, and starts on a multiple of ``align`` bytes."""
+
+    if not t.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor: the kernels have no other path")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{name} is on {t.device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+    if t.data_ptr() % align:
+        raise KernelError(f"{name} must start on a multiple of {align} bytes")
+
+
 def tag(dtype: torch.dtype) -> int:
     try:
         return DTYPE_TAG[dtype]

@@ -1,0 +1,205 @@
+"""What the page-table and chosen-page operators refuse, on the host and before anything is launched; their plain forms."""
+
+import math
+
+import pytest
+import torch
+
+from llm_runtime_study_b200.errors import KernelError
+from llm_runtime_study_b200.ops import native, page_tables, sparse_pages
+from tests.plain import sparse_pages_plain as plain
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The operators with CPU tensors taken for CUDA ones; a launch is an error of the test."""
+
+    def require(t, name, *, dtype=None, shape=None, dims=None):
+        if not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous")
+        if dtype is not None and t.dtype not in (dtype if isinstance(dtype, (tuple, list)) else (dtype,)):
+            raise KernelError(f"{name} has dtype {t.dtype}")
+        if dims is not None and t.dim() != dims:
+            raise KernelError(f"{name} has {t.dim()} dimensions")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise KernelError(f"{name} has shape {tuple(t.shape)}")
+        return t
+
+    def here(t, name, align=4):
+        if t.data_ptr() % align:
+            raise KernelError(f"{name} must start on a multiple of {align} bytes")
+
+    launched = []
+    for module in (page_tables, sparse_pages):
+        monkeypatch.setattr(module, "require", require)
+        monkeypatch.setattr(module, "stream_ptr" if module is sparse_pages else "ptr", lambda *a: 0)
+    monkeypatch.setattr(sparse_pages, "require_here", here)
+    monkeypatch.setattr(native, "require_here", here)
+    monkeypatch.setattr(native, "stream_ptr", lambda: 0)
+    monkeypatch.setattr(native, "call", lambda *a, **k: launched.append(a[0]))
+    return launched
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def good():
+    return dict(q=torch.zeros(3, 4, 64), keys=torch.zeros(5, 2, 8, 64), values=torch.zeros(5, 2, 8, 64), bounds=torch.zeros(5, 2, 2, 64),
+                chosen=ints(3, 2, 6), positions=ints(3), token_entry=ints(3), block_table=ints(2, 9), q_start=ints(3), kv_len=ints(2))
+
+
+def _bounds(a):
+    sparse_pages.page_bounds(a["keys"], a["bounds"], block_table=a["block_table"], q_start=a["q_start"], kv_len=a["kv_len"],
+                             max_q_len=a.get("max_q_len", 2))
+
+
+def _choose(a):
+    return sparse_pages.choose_pages(a["q"], a["bounds"], positions=a["positions"], token_entry=a["token_entry"],
+                                     block_table=a["block_table"], page_size=a.get("page_size", 8), budget=a.get("budget", 4),
+                                     first=a.get("first", 1), last=a.get("last", 1))
+
+
+def _attend(a):
+    return sparse_pages.paged_attention_chosen(a["q"], a["keys"], a["values"], a["chosen"], positions=a["positions"],
+                                               token_entry=a["token_entry"], block_table=a["block_table"], scale=0.1)
+
+
+def test_good_arguments_are_launched(host):
+    _bounds(good())
+    assert _choose(good()).shape == (3, 2, 4)
+    assert _attend(good()).shape == (3, 4, 64)
+    assert host == ["b200_page_bounds", "b200_choose_pages", "b200_attend_chosen"]
+    empty = good() | dict(q=torch.zeros(0, 4, 64), chosen=ints(0, 2, 6), positions=ints(0), token_entry=ints(0))
+    assert _choose(empty).shape == (0, 2, 4) and _attend(empty).shape == (0, 4, 64)
+    _bounds(good() | dict(max_q_len=0))
+    assert len(host) == 3                     # nothing to do is nothing launched
+
+
+MISALIGNED = torch.zeros(3 * 4 * 64 + 1)[1:].view(3, 4, 64)
+REFUSED = [
+    (_bounds, dict(keys=torch.zeros(5, 2, 8, 24), bounds=torch.zeros(5, 2, 2, 24))),
+    (_bounds, dict(keys=torch.zeros(5, 2, 8, 272), bounds=torch.zeros(5, 2, 2, 272))),
+    (_bounds, dict(keys=torch.zeros(5, 2, 8, 64, dtype=torch.float16))),
+    (_bounds, dict(keys=torch.zeros(0, 2, 8, 64), bounds=torch.zeros(0, 2, 2, 64))),
+    (_bounds, dict(bounds=torch.zeros(5, 2, 2, 64, dtype=torch.bfloat16))),
+    (_bounds, dict(bounds=torch.zeros(5, 2, 64))),
+    (_bounds, dict(bounds=torch.zeros(4, 2, 2, 64))),
+    (_bounds, dict(kv_len=ints(3))),
+    (_bounds, dict(kv_len=ints(2).long())),
+    (_bounds, dict(q_start=ints(2))),
+    (_bounds, dict(block_table=ints(3, 9))),
+    (_bounds, dict(block_table=ints(2, 0))),
+    (_bounds, dict(max_q_len=-1)),
+    (_bounds, dict(keys=torch.zeros(5, 8, 2, 64).transpose(1, 2))),
+    (_choose, dict(q=torch.zeros(3, 5, 64))),
+    (_choose, dict(q=torch.zeros(3, 0, 64))),
+    (_choose, dict(q=torch.zeros(3, 4, 32))),
+    (_choose, dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16))),
+    (_choose, dict(q=torch.zeros(4, 3, 64).transpose(0, 1))),
+    (_choose, dict(q=MISALIGNED)),
+    (_choose, dict(bounds=torch.zeros(5, 2, 3, 64))),
+    (_choose, dict(positions=ints(2))),
+    (_choose, dict(token_entry=ints(4))),
+    (_choose, dict(positions=ints(3).long())),
+    (_choose, dict(block_table=ints(9))),
+    (_choose, dict(block_table=ints(0, 9))),
+    (_choose, dict(block_table=ints(2, sparse_pages.MAX_TABLE_WIDTH + 1))),
+    (_choose, dict(page_size=0)),
+    (_choose, dict(budget=1)),
+    (_choose, dict(budget=3, first=2, last=2)),
+    (_choose, dict(last=0)),
+    (_choose, dict(first=-1)),
+    (_attend, dict(values=torch.zeros(5, 2, 8, 32))),
+    (_attend, dict(values=torch.zeros(5, 2, 8, 64, dtype=torch.bfloat16))),
+    (_attend, dict(chosen=ints(3, 1, 6))),
+    (_attend, dict(chosen=ints(2, 2, 6))),
+    (_attend, dict(chosen=ints(3, 2, 0))),
+    (_attend, dict(chosen=ints(3, 2, 6).long())),
+    (_attend, dict(q=MISALIGNED)),
+    (_attend, dict(keys=torch.zeros(5, 3, 8, 64), values=torch.zeros(5, 3, 8, 64))),
+    (_attend, dict(positions=ints(4))),
+]
+
+
+@pytest.mark.parametrize("at", range(len(REFUSED)))
+def test_what_does_not_fit_is_refused_before_a_launch(host, at):
+    call, change = REFUSED[at]
+    with pytest.raises(KernelError):
+        call(good() | change)
+    assert host == []
+
+
+def test_page_tables_refuse_what_does_not_fit(host):
+    tables = ints(3, 4)
+
+    def maps(**change):
+        given = dict(slots=ints(2), kv_len=ints(2), counts=ints(2), page_size=8, num_tokens=4) | change
+        return page_tables.step_maps(given.pop("tables", tables), **given)
+
+    assert maps().block_table.shape == (2, 4) and maps(width=2).block_table.shape == (2, 2)
+    assert host == ["b200_step_maps"] * 2
+    host.clear()
+    made = page_tables.StepMaps(ints(2, 4), ints(3), ints(4), ints(4), ints(4).long())
+    for change in (dict(tables=ints(3)), dict(tables=ints(0, 4)), dict(tables=tables.long()), dict(slots=ints(3)), dict(counts=ints(1)),
+                   dict(kv_len=ints(2).long()), dict(page_size=0), dict(num_tokens=-1), dict(width=0), dict(width=3, out=made),
+                   dict(num_tokens=5, out=made), dict(tables=ints(4, 3).T)):
+        with pytest.raises(KernelError):
+            maps(**change)
+    for name, value in (("block_table", ints(1, 4)), ("block_table", ints(8)), ("q_start", ints(2)), ("positions", ints(4).long()),
+                        ("token_entry", ints(3)), ("slot_map", ints(4))):
+        out = page_tables.StepMaps(**(vars(made) | {name: value}))
+        with pytest.raises(KernelError):
+            maps(out=out)
+    for change in (dict(tables=ints(0, 0)), dict(columns=ints(1)), dict(pages=ints(2).long()), dict(rows=ints(2, 1))):
+        given = dict(rows=ints(2), columns=ints(2), pages=ints(2)) | change
+        with pytest.raises(KernelError):
+            page_tables.page_table_set(given.pop("tables", tables), **given)
+    assert host == []
+
+
+def test_cpu_tensors_are_refused():
+    for call in (_bounds, _choose, _attend):
+        with pytest.raises(KernelError, match="CUDA"):
+            call(good())
+    with pytest.raises(KernelError, match="CUDA"):
+        page_tables.page_table_set(ints(3, 4), rows=ints(1), columns=ints(1), pages=ints(1))
+    with pytest.raises(KernelError, match="CUDA"):
+        page_tables.step_maps(ints(3, 4), slots=ints(1), kv_len=ints(1), counts=ints(1), page_size=8, num_tokens=1)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    class Elsewhere:
+        is_cuda, device = True, torch.device("cuda", 1)
+
+        def data_ptr(self):
+            return 64
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    with pytest.raises(KernelError, match="current device"):
+        native.require_here(Elsewhere(), "q")
+    Elsewhere.device = torch.device("cuda", 0)
+    native.require_here(Elsewhere(), "q", 16)
+    with pytest.raises(KernelError, match="multiple"):
+        native.require_here(Elsewhere(), "q", 128)
+
+
+def test_a_page_s_score_bounds_the_scores_of_its_keys():
+    g = torch.Generator().manual_seed(0)
+    keys = torch.randn(6, 1, 8, 16, generator=g, dtype=torch.float64)
+    q = torch.randn(1, 3, 16, generator=g, dtype=torch.float64)
+    low, high = keys.amin(2), keys.amax(2)
+    score = torch.maximum(q[0, :, None] * low[:, 0], q[0, :, None] * high[:, 0]).sum(-1)
+    assert bool((score[:, :, None] >= torch.einsum("hd,psd->hps", q[0], keys[:, 0]) - 1e-12).all())
+    together = high[:, 0] @ q[0].clamp(min=0).sum(0) + low[:, 0] @ q[0].clamp(max=0).sum(0)
+    torch.testing.assert_close(together, score.sum(0))
+    assert not math.isnan(float(score.sum()))
+
+
+def test_plain_choice_keeps_the_first_and_the_last_pages():
+    q, bounds = torch.ones(1, 1, 16), torch.zeros(9, 1, 2, 16)
+    bounds[4, 0, 1] = 5.0
+    table = torch.arange(9, dtype=torch.int32)[None]
+    at = torch.tensor([70]), torch.tensor([0])
+    assert plain.choose_pages(q, bounds, *at, table, 8, 4, 1, 2).tolist() == [[[0, 4, 7, 8]]]
+    assert plain.choose_pages(q, bounds, *at, table, 8, 5, 1, 2).tolist() == [[[0, 1, 4, 7, 8]]]
