@@ -1,5 +1,5 @@
-// Attention of a query over the pages of its cache that matter to it: bounds of a page's keys, choice of pages by a cheap
-// score, attention over the chosen ones.  One build per head size (HEAD_DIM).
+// Which pages of its cache matter to a query: bounds of a page's keys, choice of pages by a cheap score.  One build per head
+// size (HEAD_DIM).
 //
 //   bounds:  low_c(P) = min over the keys k of page P of k_c,   high_c(P) = max
 //   score:   s(P) = sum over the heads h of a group and the channels c of max(q_hc low_c, q_hc high_c),
@@ -8,30 +8,12 @@
 //            U = sum_h max(q_h, 0), D = sum_h min(q_h, 0): 2 HEAD_DIM products a page, however many heads the group has.
 //   choice:  the first `first` and the last `last` pages that a row sees, of the others those with the highest scores, `budget`
 //            in all; of equal scores the lower page.
-//   output:  softmax(scale q.k) over the keys of the chosen pages at positions up to the row's own.
+//   (sparse_attention.cu: softmax(scale q.k) over the keys of the chosen pages at positions up to the row's own.)
 //
 // Pages are [page][kv head][slot][HEAD_DIM], bounds [page][kv head][low, high][HEAD_DIM], both in the cache's type.
-#include <math_constants.h>
-
-#include "common.cuh"
-#include "mma.cuh"
-
-#ifndef HEAD_DIM
-#error "HEAD_DIM must be given"
-#endif
+#include "sparse_pages.cuh"
 
 namespace b200 {
-
-constexpr int kDim = HEAD_DIM;
-static_assert(kDim % 16 == 0 && kDim >= 16 && kDim <= 256, "head sizes in steps of 16 up to 256");
-
-// How a row of HEAD_DIM values is spread over lanes: 16-byte chunks, chunk i of lane l is l + i * lanes.
-template <typename T> struct RowLanes {
-  static constexpr int chunks = kDim * static_cast<int>(sizeof(T)) / 16;
-  static constexpr int lanes = chunks % 8 == 0 ? 8 : (chunks % 4 == 0 ? 4 : 2);
-  static constexpr int per_lane = chunks / lanes;
-  static constexpr int values = per_lane * Vec<T>::n;      // channels a lane holds
-};
 
 template <typename T> __device__ __forceinline__ T min_nan(T a, T b);
 template <typename T> __device__ __forceinline__ T max_nan(T a, T b);
@@ -264,131 +246,6 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads) choose_p
   select_pages(keys, seen, a.budget, a.chosen + static_cast<size_t>(blockIdx.x) * a.budget, scratch);
 }
 
-// -------------------------------------------------------------------------------------------------------- attention
-struct AttendArgs {
-  const void* q;
-  const void* keys;
-  const void* values;
-  const int* chosen;
-  const int* positions;
-  const int* token_entry;
-  const int* block_table;
-  void* out;
-  int table_width, rows, entries, q_heads, kv_heads, page_size, num_pages, budget;
-  float scale;
-};
-
-constexpr int kStreamThreads = 128;
-
-// CUDA-core attention: a few lanes hold a key's row, each such team walks keys of its own with its own running maximum, sum
-// and weighted values, which are joined at the end.  Which keys a team takes, and the order of every sum, depend on the list of
-// pages alone.
-template <typename T> struct Streams {
-  using R = RowLanes<T>;
-  static constexpr int heads = R::values <= 16 ? 4 : (R::values <= 32 ? 2 : 1);     // query heads a CTA takes
-  static constexpr int per_warp = 32 / R::lanes;
-  static constexpr int warps = kStreamThreads / 32;
-};
-
-template <typename T> __global__ void __launch_bounds__(kStreamThreads) attend_streams_kernel(const __grid_constant__ AttendArgs a) {
-  using L = Vec<T>;
-  using S = Streams<T>;
-  using R = RowLanes<T>;
-  constexpr int H = S::heads, V = R::values;
-  __shared__ float joined[S::warps][H][kDim];
-  __shared__ float joined_max[S::warps][H], joined_sum[S::warps][H];
-  pdl_trigger();
-  pdl_wait();
-  const int group = a.q_heads / a.kv_heads, slices = (group + H - 1) / H;
-  const int slice = blockIdx.x % slices, head = blockIdx.x / slices % a.kv_heads, row = blockIdx.x / slices / a.kv_heads;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, part = t % R::lanes, team = t / R::lanes;
-  const int heads_here = min(H, group - slice * H);
-  const int entry = a.token_entry[row], position = a.positions[row];
-  const bool stands = position >= 0 && entry >= 0 && entry < a.entries;
-  const int* table = a.block_table + static_cast<size_t>(stands ? entry : 0) * a.table_width;
-  const int* chosen = a.chosen + (static_cast<size_t>(row) * a.kv_heads + head) * a.budget;
-  const size_t q_row = (static_cast<size_t>(row) * a.q_heads + head * group + slice * H) * kDim;
-  float q[H][V], o[H][V], m[H], l[H];
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    m[h] = -CUDART_INF_F, l[h] = 0.f;
-#pragma unroll
-    for (int i = 0; i < R::per_lane; ++i) {
-      float v[L::n];
-      if (h < heads_here) {
-        L::unpack(reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + q_row + h * kDim)[part + i * R::lanes], v);
-      }
-#pragma unroll
-      for (int j = 0; j < L::n; ++j) q[h][i * L::n + j] = h < heads_here ? v[j] * (a.scale * 1.44269504088896340736f) : 0.f, o[h][i * L::n + j] = 0.f;
-    }
-  }
-  const int per_team = kStreamThreads / R::lanes;
-  const int listed = stands ? a.budget * a.page_size : 0;
-  for (int i = team; i < listed; i += per_team) {
-    const int place = i / a.page_size, slot = i - place * a.page_size, column = chosen[place];
-    const long long at = static_cast<long long>(column) * a.page_size + slot;
-    if (column < 0 || column >= a.table_width || at > position) continue;
-    const int page = table[column];
-    if (page < 0 || page >= a.num_pages) continue;
-    const size_t base = ((static_cast<size_t>(page) * a.kv_heads + head) * a.page_size + slot) * kDim;
-    const typename L::type* k = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.keys) + base);
-    const typename L::type* v = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.values) + base);
-    float kf[V], vf[V];
-#pragma unroll
-    for (int c = 0; c < R::per_lane; ++c) L::unpack(k[part + c * R::lanes], kf + c * L::n);
-#pragma unroll
-    for (int c = 0; c < R::per_lane; ++c) L::unpack(v[part + c * R::lanes], vf + c * L::n);
-    const unsigned team_lanes = (R::lanes == 32 ? 0xffffffffu : ((1u << R::lanes) - 1u)) << (lane / R::lanes * R::lanes);
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < V; ++c) s = fmaf(q[h][c], kf[c], s);
-#pragma unroll
-      for (int w = 1; w < R::lanes; w <<= 1) s += __shfl_xor_sync(team_lanes, s, w);
-      const float top = fmaxf(m[h], s);
-      const float keep = m[h] == top ? 1.f : exp2f(m[h] - top);
-      const float p = s == -CUDART_INF_F ? 0.f : exp2f(s - top);
-      m[h] = top;
-      l[h] = l[h] * keep + p;
-#pragma unroll
-      for (int c = 0; c < V; ++c) o[h][c] = fmaf(p, vf[c], o[h][c] * keep);
-    }
-  }
-  __syncwarp();
-  // the warp's teams, then the CTA's warps
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    float top = m[h];
-#pragma unroll
-    for (int w = R::lanes; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    const float factor = m[h] == -CUDART_INF_F ? 0.f : exp2f(m[h] - top);
-    float sum = l[h] == 0.f ? 0.f : l[h] * factor;
-#pragma unroll
-    for (int w = R::lanes; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-#pragma unroll
-    for (int c = 0; c < V; ++c) {
-      float x = o[h][c] * factor;
-#pragma unroll
-      for (int w = R::lanes; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      if (lane < R::lanes) joined[warp][h][(part + c / L::n * R::lanes) * L::n + c % L::n] = x;
-    }
-    if (lane == 0) joined_max[warp][h] = top, joined_sum[warp][h] = sum;
-  }
-  __syncthreads();
-  for (int i = t; i < heads_here * kDim; i += kStreamThreads) {
-    const int h = i / kDim, c = i % kDim;
-    float top = -CUDART_INF_F, sum = 0.f, x = 0.f;
-    for (int w = 0; w < S::warps; ++w) top = fmaxf(top, joined_max[w][h]);
-    for (int w = 0; w < S::warps; ++w) {
-      const float factor = joined_max[w][h] == -CUDART_INF_F ? 0.f : exp2f(joined_max[w][h] - top);
-      sum = fmaf(joined_sum[w][h], factor, sum);
-      x = fmaf(joined[w][h][c], factor, x);
-    }
-    static_cast<T*>(a.out)[q_row + i] = from_float<T>(sum == 0.f ? 0.f : x / sum);
-  }
-}
-
 template <typename T> int launch_bounds_kernel(const BoundsArgs& a, int max_full, cudaStream_t stream) {
   const int blocks = (max_full * a.kv_heads + 3) / 4;
   launch(page_bounds_kernel<T>, dim3(blocks, a.entries), dim3(128), 0, stream, a);
@@ -401,12 +258,6 @@ template <typename T> int launch_choose(const ChooseArgs& a, cudaStream_t stream
   if (bytes > 200 * 1024) return B200_ERR_TOO_LARGE;
   if (const int status = configure_once(once, choose_pages_kernel<T>, 200 * 1024)) return status;
   launch(choose_pages_kernel<T>, dim3(a.rows * a.kv_heads), dim3(kChooseThreads), bytes, stream, a);
-  return launch_status();
-}
-
-template <typename T> int launch_attend(const AttendArgs& a, cudaStream_t stream) {
-  const int slices = (a.q_heads / a.kv_heads + Streams<T>::heads - 1) / Streams<T>::heads;
-  launch(attend_streams_kernel<T>, dim3(a.rows * a.kv_heads * slices), dim3(kStreamThreads), 0, stream, a);
   return launch_status();
 }
 
@@ -435,18 +286,5 @@ extern "C" int b200_choose_pages(const void* q, const void* bounds, const int* p
   ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, table_width, rows, entries, q_heads, kv_heads, page_size,
                num_pages, budget, first, last};
   B200_DISPATCH_DTYPE(dtype, T, return launch_choose<T>(a, stream));
-  return 0;
-}
-
-extern "C" int b200_attend_chosen(const void* q, const void* keys, const void* values, const int* chosen, const int* positions,
-                                  const int* token_entry, const int* block_table, int table_width, void* out, int rows, int entries,
-                                  int q_heads, int kv_heads, int page_size, int num_pages, int budget, float scale, int dtype,
-                                  cudaStream_t stream) {
-  if (rows <= 0) return 0;
-  if (table_width <= 0 || entries <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || page_size <= 0 || num_pages <= 0 ||
-      budget <= 0 || static_cast<long long>(budget) * page_size > (1ll << 30)) return B200_ERR_BAD_SIZE;
-  AttendArgs a{q, keys, values, chosen, positions, token_entry, block_table, out, table_width, rows, entries, q_heads, kv_heads,
-               page_size, num_pages, budget, scale};
-  B200_DISPATCH_DTYPE(dtype, T, return launch_attend<T>(a, stream));
   return 0;
 }

@@ -1,4 +1,5 @@
-"""Attention over the pages of the cache that a query chooses by a cheap score (csrc/sparse_pages.cu), one build per head size.
+"""Attention over the pages of the cache that a query chooses by a cheap score (csrc/sparse_pages.cu, csrc/sparse_attention.cu), one build
+per head size.
 
 ``page_bounds`` keeps, beside the pages of keys, the least and the greatest value of every channel on each full page;
 ``choose_pages`` ranks the pages a query row sees by an upper bound of its scores on them; ``paged_attention_chosen`` attends
@@ -18,8 +19,9 @@ _TABLE = {
     "b200_sparse_pages_head_dim": [],
     "b200_page_bounds": [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 6 + [c_void_p],
     "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 10 + [c_void_p],
-    "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_void_p],
+    "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p],
 }
+SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
 DTYPES = (torch.float32, torch.bfloat16)
 MAX_TABLE_WIDTH = 51200      # pages of a row whose scores fit into a CTA's shared memory
 
@@ -33,7 +35,7 @@ def library_name(head_dim: int) -> str:
         raise KernelError(f"head size {head_dim} is not a multiple of 16 up to 256")
     name = f"b200_sparse_pages_d{head_dim}"
     if name not in native.library_specs():
-        native.register_library(name, ("sparse_pages.cu",), _TABLE, defines=(f"HEAD_DIM={head_dim}",))
+        native.register_library(name, SOURCES, _TABLE, defines=(f"HEAD_DIM={head_dim}",))
     return name
 
 
@@ -43,7 +45,7 @@ def build(head_dim: int) -> None:
     from ..csrc.build import build_library
 
     name = library_name(head_dim)
-    build_library(name, ("sparse_pages.cu",), native.library_defines(name))
+    build_library(name, SOURCES, native.library_defines(name))
 
 
 def _pool(t: torch.Tensor, name: str, dims: int, dtype=None) -> tuple[int, ...]:
@@ -133,6 +135,21 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
     return chosen
 
 
+def attention_parts(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> int:
+    """Into how many CTAs of a cluster the list of a row and kv head is cut: 1, 2, 4 or 8.  float32: from the list's length alone, so
+    that the order of the sums does not depend on the batch.  bfloat16: until the GPU is full, no part shorter than 128 keys."""
+
+    keys, parts = budget * page_size, 1
+    if dtype == torch.float32:
+        while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 256:
+            parts *= 2
+        return parts
+    ctas = rows * kv_heads * -(-(heads // kv_heads) // 8)
+    while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128 and 2 * parts * ctas <= 2 * native.sm_count():
+        parts *= 2
+    return parts
+
+
 def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, chosen: torch.Tensor, *, positions: torch.Tensor,
                            token_entry: torch.Tensor, block_table: torch.Tensor, scale: float) -> torch.Tensor:
     """Attention of row ``i`` of ``q`` ``[n, heads, d]`` over the keys of the pages ``chosen[i, kv head]`` (columns of row
@@ -156,5 +173,6 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     if n:
         native.call("b200_attend_chosen", ptr(q), ptr(keys), ptr(values), ptr(chosen), ptr(positions), ptr(token_entry), ptr(block_table),
                     block_table.shape[1], ptr(out), n, block_table.shape[0], heads, kv_heads, page_size, pages, chosen.shape[2],
-                    float(scale), tag(q.dtype), stream_ptr(), library=library)
+                    float(scale), attention_parts(n, heads, kv_heads, chosen.shape[2], page_size, q.dtype), tag(q.dtype), stream_ptr(),
+                    library=library)
     return out

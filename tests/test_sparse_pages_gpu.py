@@ -254,6 +254,7 @@ ATTENTION = [
     ([222, 99], [5, 1], 7, 7, 80, 8, 11),
     ([150], [2], 34, 2, 96, 16, 8),
     ([400], [1], 16, 2, 112, 24, 9),
+    ([5000], [1], 16, 2, 64, 4, 600),
 ]
 
 
