@@ -18,7 +18,7 @@ from .native import c_float, c_int, c_void_p, ptr, require, require_here, stream
 _TABLE = {
     "b200_sparse_pages_head_dim": [],
     "b200_page_bounds": [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 6 + [c_void_p],
-    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 10 + [c_void_p],
+    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 12 + [c_void_p],
     "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p],
 }
 SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
@@ -104,6 +104,24 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
                 -(-max_q_len // page_size), kv_heads, page_size, pages, tag(keys.dtype), stream_ptr(), library=library)
 
 
+def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[int, int]:
+    """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each; a cluster shares out
+    the pages of few rows, and the shared memory that the scores of many pages need."""
+
+    def fill(units: int, cluster: int) -> int:
+        while cluster < 8 and 2 * cluster * units <= 2 * native.sm_count() and width // (2 * cluster) >= 64:
+            cluster *= 2
+        return cluster
+
+    if rows >= 2 * entries:
+        sums, cluster = 2 * head_dim * 64, 1
+        while cluster < 8 and sums + 32 * width // cluster > 100 * 1024:
+            cluster *= 2
+        if sums + 32 * width // cluster <= 200 * 1024:
+            return 1, fill(-(-rows // 8) * kv_heads, cluster)
+    return 0, fill(rows * kv_heads, 1)
+
+
 def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor,
                  page_size: int, budget: int, first: int = 1, last: int = 1) -> torch.Tensor:
     """For every row of ``q`` ``[n, heads, d]`` and every kv head, which of the pages ``0 .. positions[i] // page_size`` of entry
@@ -131,7 +149,7 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
     if n:
         native.call("b200_choose_pages", ptr(q), ptr(bounds), ptr(positions), ptr(token_entry), ptr(block_table), block_table.shape[1],
                     ptr(chosen), n, block_table.shape[0], heads, kv_heads, int(page_size), pages, int(budget), int(first), int(last),
-                    tag(q.dtype), stream_ptr(), library=library)
+                    *choose_shape(n, block_table.shape[0], kv_heads, block_table.shape[1], d), tag(q.dtype), stream_ptr(), library=library)
     return chosen
 
 
