@@ -23,6 +23,7 @@ from ..errors import KVCacheError
 from ..parts.base import FixedState, PagedTensors
 from .pages import PageAllocator
 from .slots import SlotTable
+from .tables import DeviceTables
 
 
 @dataclass(frozen=True)
@@ -123,6 +124,11 @@ class GroupPool:
             name: torch.zeros((len(group.layers), *pool_shape(tuple(shape), num_pages, page_size)), dtype=dtype, device=device)
             for name, shape in group.requirement.tensors
         }
+        # one row per page, whatever the page's length
+        self.tensors.update({
+            name: torch.zeros((len(group.layers), num_pages, *shape), dtype=dtype, device=device)
+            for name, shape in group.requirement.page_tensors
+        })
         self.allocator = PageAllocator(num_pages)
         elements = sum(int(torch.tensor(shape).prod()) for _, shape in group.requirement.tensors)
         self.bytes_per_token = len(group.layers) * elements * torch.empty((), dtype=dtype).element_size()
@@ -233,6 +239,11 @@ class CacheManager:
         for s in layout.states:
             self._layer_states.setdefault(s.layer, {})[s.requirement.name] = self.state_arrays[s.key]
         self.slots = SlotTable(max_requests, self.device)
+        # the block tables of all slots, on a device that runs kernels
+        self.tables: DeviceTables | None = None
+        if self.device.type == "cuda" and self.groups:
+            widths = [-(-pool.pages_for(self.max_seq_len) // 4) * 4 for pool in self.groups]
+            self.tables = DeviceTables(max_requests, widths, self.device)
         self._layer_group = {layer: (g, i) for g, group in enumerate(layout.groups) for i, layer in enumerate(group.layers)}
         self._free_slots = list(range(max_requests - 1, -1, -1))
         self._active: dict[int, RequestCache] = {}

@@ -8,7 +8,7 @@ with 2.  Added here: ``--prompt-ids`` (the prompt as token ids: the engine prope
 starts at token ids, and a folder of random weights has no tokenizer),
 ``--random-weights CONFIG`` with ``--weights-seed`` (write a model folder with seeded
 random weights into ``--model`` first), ``--max-batch-size``, ``--page-size``,
-``--max-tokens-per-step``, ``--no-cuda-graph``, ``--any-storage-dtype``.
+``--max-tokens-per-step``, ``--attention-pages``, ``--no-cuda-graph``, ``--any-storage-dtype``.
 
 The program is a thin shell around one ``Session``: it loads an ``Engine`` once, turns
 every prompt into token ids, submits it to a scheduler of the engine and consumes that
@@ -64,6 +64,8 @@ def build_parser() -> argparse.ArgumentParser:
     add("--max-batch-size", type=int, default=1)
     add("--page-size", type=int, default=16)
     add("--max-tokens-per-step", type=int, default=2048)
+    add("--attention-pages", type=int, metavar="N",
+        help="read at most N pages of keys and values for a token, the ones that can matter most to it (default: all)")
     add("--no-cuda-graph", action="store_true")
     add("--any-storage-dtype", action="store_true",
         help="accept weights stored in another floating type than config.json's torch_dtype")
@@ -110,6 +112,7 @@ class Session:
             args.model, device=args.device, dtype=args.dtype, max_seq_len=args.max_seq_len,
             max_batch_size=args.max_batch_size, use_cuda_graph=not args.no_cuda_graph, page_size=args.page_size,
             max_tokens_per_step=args.max_tokens_per_step, strict_dtype=not args.any_storage_dtype,
+            attention_pages=args.attention_pages,
         )
         self.load_host_mib = max(0.0, _peak_host_mib() - before)
         self.has_text = self.engine.tokenizer is not None

@@ -12,6 +12,7 @@
 //
 // Nothing but copies of a few bytes per token and column: what bounds it is the launch.
 #include "common.cuh"
+#include "slots.h"
 
 namespace b200 {
 
@@ -43,21 +44,10 @@ struct StepMapsArgs {
 constexpr int kMapThreads = 256;
 constexpr int kMapShare = 4 * kMapThreads;     // columns, and tokens, of an entry that one CTA takes at a time
 
-// One CTA per (entry, share of its columns and tokens).  The tokens before an entry are counted by every CTA itself (a step
-// has at most some hundred entries), so no CTA waits for another.  VEC: four columns to a 16-byte access.
+// out[c] = row[c] for the columns below `held`, -1 behind them; VEC: four columns to a 16-byte access.
 template <bool VEC>
-__global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const __grid_constant__ StepMapsArgs a) {
-  __shared__ int warp_sums[kMapThreads / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int r = blockIdx.x, t = threadIdx.x;
-  const int slot = a.slots[r];
-  const bool known = slot >= 0 && slot < a.table_rows;
-  const int* row = a.tables + static_cast<size_t>(known ? slot : 0) * a.width;
-  const int length = max(a.kv_len[r], 0), page_size = a.page_size;
-  const int held = known && length > 0 ? min((length - 1) / page_size + 1, a.width) : 0;      // columns that hold a page
-  int* out = a.block_table + static_cast<size_t>(r) * a.out_width;
-  for (int c = (blockIdx.y * kMapThreads + t) * 4; c < a.out_width; c += gridDim.y * kMapShare) {
+__device__ __forceinline__ void copy_row(const int* row, int held, int* out, int out_width, int thread, int threads) {
+  for (int c = thread * 4; c < out_width; c += threads * 4) {
     if (VEC) {
       int4 v = c < held ? *reinterpret_cast<const int4*>(row + c) : make_int4(-1, -1, -1, -1);
       if (c + 1 >= held) v.y = -1;
@@ -65,9 +55,24 @@ __global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const __grid_con
       if (c + 3 >= held) v.w = -1;
       *reinterpret_cast<int4*>(out + c) = v;
     } else {
-      for (int i = c; i < min(c + 4, a.out_width); ++i) out[i] = i < held ? row[i] : -1;
+      for (int i = c; i < min(c + 4, out_width); ++i) out[i] = i < held ? row[i] : -1;
     }
   }
+}
+
+// One CTA per (entry, share of its columns and tokens).  The tokens before an entry are counted by every CTA itself (a step
+// has at most some hundred entries), so no CTA waits for another.
+template <bool VEC>
+__global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const __grid_constant__ StepMapsArgs a) {
+  __shared__ int warp_sums[kMapThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, t = threadIdx.x;
+  const int slot = a.slots[r], length = max(a.kv_len[r], 0), page_size = a.page_size;
+  const bool known = slot >= 0 && slot < a.table_rows;
+  const int* row = a.tables + static_cast<size_t>(known ? slot : 0) * a.width;
+  const int held = known && length > 0 ? min((length - 1) / page_size + 1, a.width) : 0;      // columns that hold a page
+  copy_row<VEC>(row, held, a.block_table + static_cast<size_t>(r) * a.out_width, a.out_width, blockIdx.y * kMapThreads + t, gridDim.y * kMapThreads);
   if (a.q_start == nullptr && a.positions == nullptr && a.token_entry == nullptr && a.slot_map == nullptr) return;
   int before = 0;
   for (int i = t; i < r; i += kMapThreads) before += max(a.counts[i], 0);
@@ -96,6 +101,47 @@ __global__ void __launch_bounds__(kMapThreads) step_maps_kernel(const __grid_con
   }
 }
 
+// The start of a step of single decoded tokens: what b200_slot_load does (slots.cu), and the block table's row of each entry, one
+// CTA each; the record is read before it is advanced, and by nobody else.
+struct SlotMapsArgs {
+  int* records;
+  const int* slots;
+  int* token_ids;
+  int* positions;
+  int* kv_len;
+  const int* tables;
+  int* block_table;
+  int records_count, table_rows, width, out_width, page_size;
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(kMapThreads) slot_load_maps_kernel(const __grid_constant__ SlotMapsArgs a) {
+  __shared__ int shared_length;
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x, t = threadIdx.x, slot = a.slots[r];
+  if (t == 0) {
+    int* rec = a.records + static_cast<size_t>(slot) * kSlotWords;
+    const bool live = slot >= 0 && slot < a.records_count && rec[kSlotLive] != 0;
+    const int pos = live ? rec[kSlotPosition] : 0, token = live ? rec[kSlotLastToken] : 0;
+    a.token_ids[r] = token < 0 ? 0 : token;      // a refused draw (-1: non-finite logits) is reported by the host; never index with it
+    a.positions[r] = pos;
+    a.kv_len[r] = live ? pos + 1 : 0;
+    if (live) rec[kSlotPosition] = pos + 1;
+    shared_length = live ? pos + 1 : 0;
+  }
+  __syncthreads();
+  const int length = max(shared_length, 0);
+  const bool known = slot >= 0 && slot < a.table_rows;
+  const int held = known && length > 0 ? min((length - 1) / a.page_size + 1, a.width) : 0;
+  copy_row<VEC>(a.tables + static_cast<size_t>(known ? slot : 0) * a.width, held, a.block_table + static_cast<size_t>(r) * a.out_width,
+                a.out_width, t, kMapThreads);
+}
+
+bool vector_rows(const int* tables, int width, const int* block_table, int out_width) {
+  return width % 4 == 0 && out_width % 4 == 0 && reinterpret_cast<uintptr_t>(tables) % 16 == 0 && reinterpret_cast<uintptr_t>(block_table) % 16 == 0;
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -117,12 +163,22 @@ extern "C" int b200_step_maps(const int* tables, int table_rows, int width, cons
   if (table_rows <= 0 || width <= 0 || out_width <= 0 || page_size <= 0 || num_tokens < 0) return B200_ERR_BAD_SIZE;
   StepMapsArgs a{tables, slots, kv_len, counts, block_table, q_start, positions, token_entry, slot_map,
                  table_rows, width, out_width, entries, page_size, num_tokens};
-  const bool vec = width % 4 == 0 && out_width % 4 == 0 && reinterpret_cast<uintptr_t>(tables) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(block_table) % 16 == 0;
+  const bool vec = vector_rows(tables, width, block_table, out_width);
   // as many shares as the wider of a row's columns and a mean entry's tokens asks for
   const int tokens = (num_tokens + entries - 1) / entries;
   int shares = ((out_width > tokens ? out_width : tokens) + kMapShare - 1) / kMapShare;
   if (shares > 64) shares = 64;
   launch(vec ? step_maps_kernel<true> : step_maps_kernel<false>, dim3(entries, shares), dim3(kMapThreads), 0, stream, a);
+  return launch_status();
+}
+
+extern "C" int b200_slot_load_maps(int* records, int records_count, const int* slots, int* token_ids, int* positions, int* kv_len,
+                                   const int* tables, int table_rows, int width, int* block_table, int out_width, int entries,
+                                   int page_size, cudaStream_t stream) {
+  if (entries <= 0) return 0;
+  if (records_count <= 0 || table_rows <= 0 || width <= 0 || out_width <= 0 || page_size <= 0) return B200_ERR_BAD_SIZE;
+  SlotMapsArgs a{records, slots, token_ids, positions, kv_len, tables, block_table, records_count, table_rows, width, out_width, page_size};
+  launch(vector_rows(tables, width, block_table, out_width) ? slot_load_maps_kernel<true> : slot_load_maps_kernel<false>, dim3(entries),
+         dim3(kMapThreads), 0, stream, a);
   return launch_status();
 }

@@ -27,6 +27,7 @@ struct AttendArgs {
 };
 
 constexpr int kPlaces = 512;       // pages of a list that a CTA looks up at a time
+constexpr int kSumsRow = kDim + 1; // a row of weighted values in shared memory: what the lanes of a fragment write falls on 32 banks
 
 struct Place {
   int page;     // page of the pool
@@ -72,7 +73,7 @@ __device__ __forceinline__ int look_up(const AttendArgs& a, const Work& w, int f
 // warps' weighted values, top[w][h] and total[w][h] their maxima and sums.  All threads of all parts; the order of every sum is
 // that of the warps and of the parts.
 template <typename T, int WARPS, int H>
-__device__ void join_and_write(const AttendArgs& a, const Work& w, float (*sums)[H][kDim], float (*top)[H], float (*total)[H], int heads_here,
+__device__ void join_and_write(const AttendArgs& a, const Work& w, float (*sums)[H][kSumsRow], float (*top)[H], float (*total)[H], int heads_here,
                                T* out) {
   __shared__ float joined_top[H], joined_total[H];
   constexpr int kThreads = WARPS * 32;
@@ -99,22 +100,24 @@ __device__ void join_and_write(const AttendArgs& a, const Work& w, float (*sums)
     }
   }
   if (a.parts == 1) return;
+  __syncthreads();                      // the cluster's barriers want whole warps
   cluster_arrive();
   cluster_wait();                       // every part's sums are in its CTA's shared memory
   const uint32_t sums_at = shared_address(&sums[0][0][0]), top_at = shared_address(joined_top), total_at = shared_address(joined_total);
   for (int i = w.part * kThreads + t; i < heads_here * kDim; i += a.parts * kThreads) {
-    const int h = i / kDim;
+    const int h = i / kDim, at = h * kSumsRow + i % kDim;
     float m = -CUDART_INF_F;
     for (int p = 0; p < a.parts; ++p) m = fmaxf(m, load_in_cluster(in_cluster(top_at + h * 4, p)));
     float x = 0.f, l = 0.f;
     for (int p = 0; p < a.parts; ++p) {
       const float own = load_in_cluster(in_cluster(top_at + h * 4, p));
       const float factor = own == -CUDART_INF_F ? 0.f : exp2f(own - m);
-      x = fmaf(load_in_cluster(in_cluster(sums_at + i * 4, p)), factor, x);
+      x = fmaf(load_in_cluster(in_cluster(sums_at + at * 4, p)), factor, x);
       l = fmaf(load_in_cluster(in_cluster(total_at + h * 4, p)), factor, l);
     }
     out[i] = from_float<T>(l == 0.f ? 0.f : x / l);
   }
+  __syncthreads();
   cluster_leave();                      // nobody leaves while its sums are being read
 }
 
@@ -131,7 +134,7 @@ struct Streams {
 __global__ void __launch_bounds__(Streams::threads) attend_streams_kernel(const __grid_constant__ AttendArgs a) {
   using R = RowLanes<float>;
   constexpr int H = Streams::heads, V = R::values, U = Streams::ahead, kWarps = Streams::threads / 32, kTeams = Streams::threads / R::lanes;
-  __shared__ float sums[kWarps][H][kDim];
+  __shared__ float sums[kWarps][H][kSumsRow];
   __shared__ float top[kWarps][H], total[kWarps][H];
   __shared__ Place places[kPlaces];
   pdl_trigger();
@@ -224,12 +227,15 @@ __global__ void __launch_bounds__(Streams::threads) attend_streams_kernel(const 
 
 // --------------------------------------------------------------------------------------------- bfloat16, tensor cores
 // S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16, keys (and value columns) as the 16 rows, the group's query heads as the 8
-// columns: a group has few heads, so this way round nothing of the 16 rows is padding.  The operands are loaded from global
-// memory straight into the fragments' registers, 16 bytes a lane and row: the sum over channels does not mind their order, so a
-// lane takes eight neighbouring channels where the fragment wants two pairs of two, twice; and the rows of O^T may be any columns,
-// so a lane takes eight neighbouring ones of each of its four keys and pairs two keys by a byte permutation.  No shared memory, no
-// barrier in the loop, and what a lane writes at the end is eight neighbouring columns.  The weights P^T are in the layout of the
-// accumulator of S^T and are turned into the operand's by a transposition of 8x8 tiles across the warp.
+// columns: a group has few heads, so this way round nothing of the 16 rows is padding.  Keys and values are loaded from global
+// memory straight into registers, 16 bytes a lane: lane (g, t) takes channels 8 t .. 8 t + 7 of every 32 of the rows g and g + 8 of
+// a tile of 16 keys.  The sum over channels does not mind their order, so these are the fragments of K where they lie.  Values
+// (and the weights P^T, which come in the layout of the accumulator) are turned by movmatrix, 8x8 numbers across the warp.  No
+// shared memory and no barrier in the loop.
+//
+// Eight neighbouring lanes load from two rows, which lie on the same banks of the L1 cache where a row is a multiple of 128 bytes;
+// odd rows then take the blocks of 32 channels of each pair in the other order and exchange the registers afterwards.  (874 prompt
+// rows, 8 kv heads, 2,048 keys each: the data stage of L1 was 91 % busy with values read by columns and both kinds on shared banks.)
 __device__ __forceinline__ uint4 load_row_16(const __nv_bfloat16* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -240,67 +246,53 @@ __device__ __forceinline__ uint2 load_row_8(const __nv_bfloat16* p) {
   asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint32_t load_row_4(const __nv_bfloat16* p) {
-  uint32_t v;
-  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];\n" : "=r"(v) : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
 
-constexpr int kKeyRegs = kDim / 8;              // registers of a lane for its channels of one key: pairs
-constexpr int kBlocks64 = kDim / 64, kBlocks32 = kDim % 64 / 32, kBlocks16 = kDim % 32 / 16;
-constexpr int kValueRegs = kDim / 16;           // for its columns of one value row
+constexpr int kRowRegs = kDim / 8;              // registers of a lane for its channels of one row: pairs
+constexpr int kTiles = kDim / 16;                // tiles of 16 value columns
+constexpr bool kSwapOdd = kDim % 64 == 0;       // rows of whole 128 bytes
 
 // A lane's channels of one row: 8 t .. 8 t + 7 of every 32, 4 t .. 4 t + 3 of the last 16.
-__device__ __forceinline__ void load_channels(uint32_t (&r)[kKeyRegs], const __nv_bfloat16* row, int t, bool is) {
+__device__ __forceinline__ void load_channels(uint32_t (&r)[kRowRegs], const __nv_bfloat16* row, int t, bool odd, bool is) {
 #pragma unroll
   for (int b = 0; b < kDim / 32; ++b) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (is) v = load_row_16(row + 32 * b + 8 * t);
+    if (is) v = load_row_16(row + 32 * (kSwapOdd && odd ? b ^ 1 : b) + 8 * t);
     r[4 * b] = v.x, r[4 * b + 1] = v.y, r[4 * b + 2] = v.z, r[4 * b + 3] = v.w;
   }
   if (kDim % 32) {
     uint2 v = make_uint2(0, 0);
     if (is) v = load_row_8(row + kDim / 32 * 32 + 4 * t);
-    r[kKeyRegs - 2] = v.x, r[kKeyRegs - 1] = v.y;
+    r[kRowRegs - 2] = v.x, r[kRowRegs - 1] = v.y;
   }
 }
-
-// A lane's columns of one value row: 8 g .. 8 g + 7 of every 64, 4 g .. 4 g + 3 of a further 32, 2 g and 2 g + 1 of the last 16.
-__device__ __forceinline__ void load_columns(uint32_t (&r)[kValueRegs], const __nv_bfloat16* row, int g, bool is) {
+// Puts the blocks of an odd row into their places.
+__device__ __forceinline__ void order_channels(uint32_t (&r)[kRowRegs], bool odd) {
+  if constexpr (kSwapOdd) {
 #pragma unroll
-  for (int b = 0; b < kBlocks64; ++b) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (is) v = load_row_16(row + 64 * b + 8 * g);
-    r[4 * b] = v.x, r[4 * b + 1] = v.y, r[4 * b + 2] = v.z, r[4 * b + 3] = v.w;
-  }
-  if (kBlocks32) {
-    uint2 v = make_uint2(0, 0);
-    if (is) v = load_row_8(row + 64 * kBlocks64 + 4 * g);
-    r[4 * kBlocks64] = v.x, r[4 * kBlocks64 + 1] = v.y;
-  }
-  if (kBlocks16) {
-    uint32_t v = 0;
-    if (is) v = load_row_4(row + 64 * kBlocks64 + 32 * kBlocks32 + 2 * g);
-    r[kValueRegs - 1] = v;
+    for (int i = 0; i < kRowRegs / 2; ++i) {
+      const int a = i / 4 * 8 + i % 4, b = a + 4;
+      const uint32_t x = r[a], y = r[b];
+      r[a] = odd ? y : x, r[b] = odd ? x : y;
+    }
   }
 }
-// The first of the two columns that register i of a lane's value row holds.
-__device__ __forceinline__ int column_of(int i, int g) {
-  if (i < 4 * kBlocks64) return 64 * (i / 4) + 8 * g + 2 * (i % 4);
-  if (kBlocks32 && i < 4 * kBlocks64 + 2) return 64 * kBlocks64 + 4 * g + 2 * (i - 4 * kBlocks64);
-  return 64 * kBlocks64 + 32 * kBlocks32 + 2 * g;
+// The column that row g (half 0) or g + 8 (half 1) of tile m of O^T stands for: registers 2 m and 2 m + 1 of a lane hold columns of
+// which the transposition hands two neighbours to neighbouring rows.
+__device__ __forceinline__ int column_of(int m, int half, int g) {
+  if (kDim % 32 && m == kDim / 16 - 1) return 16 * m + 4 * (g >> 1) + 2 * half + (g & 1);
+  return 32 * (m / 2) + 8 * (g >> 1) + 4 * (m % 2) + 2 * half + (g & 1);
 }
 
 // NT: tiles of eight query heads of a CTA.  WHOLE: pages are whole tiles of 16 keys, so that a tile is a run of rows.
 template <int NT, int WARPS, bool WHOLE>
 __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int H = 8 * NT;
-  __shared__ float sums[WARPS][H][kDim];
+  __shared__ float sums[WARPS][H][kSumsRow];
   __shared__ float top[WARPS][H], total[WARPS][H];
   __shared__ Place places[kPlaces];
   pdl_trigger();
@@ -308,19 +300,20 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
   const int group = a.q_heads / a.kv_heads;
   const Work w = work_of(a, (group + H - 1) / H);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const bool odd = g & 1;
   const int heads_here = min(H, group - w.slice * H);
   const int entry = a.token_entry[w.row], position = a.positions[w.row];
   const bool stands = position >= 0 && entry >= 0 && entry < a.entries;
   const size_t q_row = (static_cast<size_t>(w.row) * a.q_heads + w.head * group + w.slice * H) * kDim;
-  uint32_t q[NT][kKeyRegs];
+  uint32_t q[NT][kRowRegs];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) load_channels(q[n], static_cast<const __nv_bfloat16*>(a.q) + q_row + (8 * n + g) * kDim, t, 8 * n + g < heads_here);
-  float o[NT][kValueRegs][4], m[NT][2], l[NT][2];
+  for (int n = 0; n < NT; ++n) load_channels(q[n], static_cast<const __nv_bfloat16*>(a.q) + q_row + (8 * n + g) * kDim, t, false, 8 * n + g < heads_here);
+  float o[NT][kTiles][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n][0] = m[n][1] = -CUDART_INF_F, l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kValueRegs; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    for (int i = 0; i < kTiles; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
   const __nv_bfloat16* keys = static_cast<const __nv_bfloat16*>(a.keys) + static_cast<size_t>(w.head) * a.page_size * kDim;
   const __nv_bfloat16* values = static_cast<const __nv_bfloat16*>(a.values) + static_cast<size_t>(w.head) * a.page_size * kDim;
@@ -332,47 +325,41 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
     const int per_place = a.page_size / 16;         // WHOLE: tiles of a page
     const int tiles = WHOLE ? count * per_place : (count * a.page_size + 15) / 16;
     for (int tile = warp; tile < tiles; tile += WARPS) {
-      // where the lane's rows lie: keys g and g + 8 of the tile, values 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-      size_t key_at[2], value_at[4];
-      bool key_is[2], value_is[4];
+      size_t at[2];        // where the lane's rows g and g + 8 lie
+      bool is[2];
       if (WHOLE) {
         const int place = tile / per_place, slot = (tile - place * per_place) * 16;
         const Place here = places[place];
         const int last = here.last - slot;
         if (last < 0) continue;                      // the same for the whole warp
-        const size_t at = here.page * page_stride + slot * kDim;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) key_at[i] = at + (g + 8 * i) * kDim, key_is[i] = g + 8 * i <= last;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) value_at[i] = at + (2 * t + i % 2 + i / 2 * 8) * kDim, value_is[i] = 2 * t + i % 2 + i / 2 * 8 <= last;
+        for (int i = 0; i < 2; ++i) at[i] = here.page * page_stride + (slot + g + 8 * i) * kDim, is[i] = g + 8 * i <= last;
       } else {
-        auto find = [&](int k, size_t& at, bool& is) {
-          const int place = k / a.page_size, slot = k - place * a.page_size;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int k = tile * 16 + g + 8 * i, place = k / a.page_size, slot = k - place * a.page_size;
           const Place here = place < count ? places[place] : Place{0, -1};
-          is = slot <= here.last;
-          at = here.page * page_stride + slot * kDim;
-        };
-#pragma unroll
-        for (int i = 0; i < 2; ++i) find(tile * 16 + g + 8 * i, key_at[i], key_is[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) find(tile * 16 + 2 * t + i % 2 + i / 2 * 8, value_at[i], value_is[i]);
+          at[i] = here.page * page_stride + slot * kDim, is[i] = slot <= here.last;
+        }
       }
-      uint32_t k0[kKeyRegs], k1[kKeyRegs], v[4][kValueRegs];
-      load_channels(k0, keys + key_at[0], t, key_is[0]);
-      load_channels(k1, keys + key_at[1], t, key_is[1]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_columns(v[i], values + value_at[i], g, value_is[i]);
+      uint32_t k0[kRowRegs], k1[kRowRegs], v0[kRowRegs], v1[kRowRegs];
+      load_channels(k0, keys + at[0], t, odd, is[0]);
+      load_channels(k1, keys + at[1], t, odd, is[1]);
+      load_channels(v0, values + at[0], t, odd, is[0]);
+      load_channels(v1, values + at[1], t, odd, is[1]);
+      order_channels(k0, odd);
+      order_channels(k1, odd);
       uint32_t weights[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float s[2][4] = {};        // two sums, so that each product waits for the one before the last
 #pragma unroll
-        for (int i = 0; i < kKeyRegs / 2; ++i) mma_bf16(s[i & 1], {k0[2 * i], k1[2 * i], k0[2 * i + 1], k1[2 * i + 1]}, q[n][2 * i], q[n][2 * i + 1]);
+        for (int i = 0; i < kRowRegs / 2; ++i) mma_bf16(s[i & 1], {k0[2 * i], k1[2 * i], k0[2 * i + 1], k1[2 * i + 1]}, q[n][2 * i], q[n][2 * i + 1]);
         float keep[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {                // heads 2 t and 2 t + 1; keys g and g + 8
-          float x = key_is[0] ? (s[0][c] + s[1][c]) * a.scale_log2 : -CUDART_INF_F;
-          float y = key_is[1] ? (s[0][2 + c] + s[1][2 + c]) * a.scale_log2 : -CUDART_INF_F;
+          float x = is[0] ? (s[0][c] + s[1][c]) * a.scale_log2 : -CUDART_INF_F;
+          float y = is[1] ? (s[0][2 + c] + s[1][2 + c]) * a.scale_log2 : -CUDART_INF_F;
           float most = fmaxf(x, y);
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
@@ -389,15 +376,16 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
         weights[n][1] = transpose_8x8(pack_bf16(s[0][2], s[0][3]));
         if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
-          for (int i = 0; i < kValueRegs; ++i) o[n][i][0] *= keep[0], o[n][i][1] *= keep[1], o[n][i][2] *= keep[0], o[n][i][3] *= keep[1];
+          for (int i = 0; i < kTiles; ++i) o[n][i][0] *= keep[0], o[n][i][1] *= keep[1], o[n][i][2] *= keep[0], o[n][i][3] *= keep[1];
         }
       }
+      order_channels(v0, odd);
+      order_channels(v1, odd);
 #pragma unroll
-      for (int i = 0; i < kValueRegs; ++i) {
-        const uint32_t pairs[4] = {__byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
-                                   __byte_perm(v[2][i], v[3][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x7632)};
+      for (int i = 0; i < kTiles; ++i) {
+        const uint32_t turned[4] = {transpose_8x8(v0[2 * i]), transpose_8x8(v0[2 * i + 1]), transpose_8x8(v1[2 * i]), transpose_8x8(v1[2 * i + 1])};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], pairs, weights[n][0], weights[n][1]);
+        for (int n = 0; n < NT; ++n) mma_bf16(o[n][i], turned, weights[n][0], weights[n][1]);
       }
     }
   }
@@ -412,7 +400,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       if (g == 0) top[warp][h] = m[n][c], total[warp][h] = sum;
 #pragma unroll
-      for (int i = 0; i < kValueRegs; ++i) *reinterpret_cast<float2*>(&sums[warp][h][column_of(i, g)]) = make_float2(o[n][i][c], o[n][i][2 + c]);
+      for (int i = 0; i < kTiles; ++i) sums[warp][h][column_of(i, 0, g)] = o[n][i][c], sums[warp][h][column_of(i, 1, g)] = o[n][i][2 + c];
     }
   }
   join_and_write<__nv_bfloat16, WARPS, H>(a, w, sums, top, total, heads_here, static_cast<__nv_bfloat16*>(a.out) + q_row);

@@ -93,6 +93,7 @@ struct ChooseArgs {
   const int* token_entry;
   const int* block_table;
   int* chosen;
+  uint32_t* keys;          // scratch of the scores of single tokens, [rows][kv_heads][table_width]
   int table_width, rows, entries, q_heads, kv_heads, page_size, num_pages, budget, first, last, cluster;
 };
 
@@ -117,36 +118,52 @@ constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
 template <int WARPS> __device__ __forceinline__ void sync_group() {
   if (WARPS == 1) __syncwarp(); else __syncthreads();
 }
-constexpr int select_words(int warps) { return 256 + 3 * warps + 2; }
+constexpr int select_words(int warps) { return 256 + 4 * warps + 3; }
 
 // The `budget` highest of keys[0 .. count) that are not kKeyNone, lower indices first among equals, written in rising order
 // of their indices; -1 behind them.  WARPS warps take part (t: the thread among them), all of the CTA's or one.
+//
+// The border is found digit by digit of eight bits, from the highest bit in which the candidates differ at all (scores lie close
+// together: their upper bits say nothing), until the keys of a digit are wanted all or none: two rounds as a rule.
 template <int WARPS> __device__ void select_pages(const uint32_t* keys, int count, int budget, int* out, uint32_t* scratch, int t) {
   constexpr int kThreads = WARPS * 32;
   uint32_t* histogram = scratch;
-  uint32_t* held = scratch + 256;              // per warp
-  uint32_t* above = held + WARPS;
-  uint32_t* equal = above + WARPS;
-  uint32_t* found = equal + WARPS;             // digit, how many are still wanted among its keys
+  uint32_t* per_warp = scratch + 256;          // four words of each
+  uint32_t* found = per_warp + 4 * WARPS;      // digit, how many are still wanted among its keys, how many those are
   const int lane = t & 31, warp = t >> 5;
-  uint32_t some = 0;
-  for (int i = t; i < count; i += kThreads) some += keys[i] != kKeyNone;
-  some = __reduce_add_sync(0xffffffffu, some);
+  uint32_t always = 0, others = 0, least = 0xffffffffu, most = 0;
+  for (int i = t; i < count; i += kThreads) {
+    const uint32_t key = keys[i];
+    if (key == kKeyAlways) ++always;
+    else if (key != kKeyNone) ++others, least = min(least, key), most = max(most, key);
+  }
+  always = __reduce_add_sync(0xffffffffu, always);
+  others = __reduce_add_sync(0xffffffffu, others);
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
   if (WARPS > 1) {
-    if (lane == 0) held[warp] = some;
+    if (lane == 0) per_warp[4 * warp] = always, per_warp[4 * warp + 1] = others, per_warp[4 * warp + 2] = least, per_warp[4 * warp + 3] = most;
     __syncthreads();
-    some = 0;
-    for (int w = 0; w < WARPS; ++w) some += held[w];
+    always = others = most = 0, least = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      always += per_warp[4 * w], others += per_warp[4 * w + 1];
+      least = min(least, per_warp[4 * w + 2]), most = max(most, per_warp[4 * w + 3]);
+    }
   }
   uint32_t threshold = 0, wanted = 0;          // take keys above the threshold, and the first `wanted` equal to it
-  if (some > static_cast<uint32_t>(budget)) {
-    wanted = budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+  if (always + others > static_cast<uint32_t>(budget)) {
+    wanted = budget - always;                  // the first and the last pages fit into every budget
+    int high = least == most ? 0 : 32 - __clz(least ^ most);       // bits below this one differ
+    threshold = wanted == 0 ? kKeyNaN : (high == 32 ? 0u : most >> high << high);
+    while (wanted > 0 && high > 0) {
+      const int low = max(high - 8, 0);
+      const uint32_t digits = (1u << (high - low)) - 1u;
       for (int i = t; i < 256; i += kThreads) histogram[i] = 0;
       sync_group<WARPS>();
       for (int i = t; i < count; i += kThreads) {
         const uint32_t key = keys[i];
-        if (key != kKeyNone && (shift == 24 || (key >> (shift + 8)) == (threshold >> (shift + 8)))) atomicAdd(&histogram[(key >> shift) & 255u], 1u);
+        if (key != kKeyNone && key != kKeyAlways && (high == 32 || key >> high == threshold >> high)) atomicAdd(&histogram[key >> low & digits], 1u);
       }
       sync_group<WARPS>();
       if (warp == 0) {       // lane l holds the digits 255 - 8 l down to 248 - 8 l
@@ -163,14 +180,19 @@ template <int WARPS> __device__ void select_pages(const uint32_t* keys, int coun
         if (before < wanted && wanted <= upto) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (before < wanted && wanted <= before + mine[i]) found[0] = 255 - 8 * lane - i, found[1] = wanted - before;
+            if (before < wanted && wanted <= before + mine[i]) found[0] = 255 - 8 * lane - i, found[1] = wanted - before, found[2] = mine[i];
             before += mine[i];
           }
         }
       }
       sync_group<WARPS>();
-      threshold |= found[0] << shift;
+      threshold |= found[0] << low;
       wanted = found[1];
+      high = low;
+      if (wanted == found[2]) {                // all keys of this digit: whatever is not below them
+        threshold = threshold > 0 ? threshold - 1 : 0;
+        wanted = 0;
+      }
     }
   }
   // each warp keeps a run of indices: count, then write at the place the warps before it leave
@@ -181,10 +203,11 @@ template <int WARPS> __device__ void select_pages(const uint32_t* keys, int coun
     for (int i = from + lane; i < to; i += 32) more += keys[i] > threshold, same += keys[i] == threshold;
     more = __reduce_add_sync(0xffffffffu, more);
     same = __reduce_add_sync(0xffffffffu, same);
-    if (lane == 0) above[warp] = more, equal[warp] = same;
+    __syncthreads();                           // the sums of above have been read
+    if (lane == 0) per_warp[2 * warp] = more, per_warp[2 * warp + 1] = same;
     __syncthreads();
     more = same = 0;
-    for (int w = 0; w < warp; ++w) more += above[w], same += equal[w];
+    for (int w = 0; w < warp; ++w) more += per_warp[2 * w], same += per_warp[2 * w + 1];
   }
   const uint32_t below = (1u << lane) - 1u;
   for (int i = from; i < to; i += 32) {
@@ -196,74 +219,97 @@ template <int WARPS> __device__ void select_pages(const uint32_t* keys, int coun
     more += __popc(greater_lanes);
     same += __popc(tie_lanes);
   }
-  const int kept = min(some, static_cast<uint32_t>(budget));
+  const int kept = min(always + others, static_cast<uint32_t>(budget));
   for (int i = kept + t; i < budget; i += kThreads) out[i] = -1;
 }
 
-// U and D of one channel (see the top of the file).  A NaN goes into both sums' score by way of D.
+// U and D (see the top of the file).  A NaN gets into the score by way of D.
+__device__ __forceinline__ void add_part(float q, double& up, double& down) {
+  if (q > 0) up += q; else down += q;
+}
 template <typename T> __device__ __forceinline__ void parts_of(const T* q, int group, double& up, double& down) {
   up = down = 0;
-  for (int h = 0; h < group; ++h) {
-    const double v = to_float<T>(q[h * kDim]);
-    if (v > 0) up += v; else down += v;
-  }
+  for (int h = 0; h < group; ++h) add_part(to_float<T>(q[h * kDim]), up, down);
 }
 
-__device__ __forceinline__ void store_in_cluster(uint32_t address, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(address), "r"(v) : "memory");
+// Whether a page is held, and whether it is read whatever its score.
+__device__ __forceinline__ bool is_held(const ChooseArgs& a, int id) { return id >= 0 && id < a.num_pages; }
+__device__ __forceinline__ uint32_t key_of(const ChooseArgs& a, int p, int seen, bool held, double score) {
+  return !held ? kKeyNone : (p < a.first || p >= seen - a.last ? kKeyAlways : score_key(score));
 }
 
-// Single tokens: a cluster per (row, kv head).  Its CTAs share out the pages; a few lanes (RowLanes) hold U and D in registers
-// and read a page's bounds 16 bytes at a time; every score's key goes into the first CTA's shared memory, which then chooses.
-// Scores are summed in 64 bits and rounded once: the products of bfloat16 numbers are exact there, so neither the order of the sum
-// nor its spread over lanes moves a page across the border.
-template <typename T> __global__ void __launch_bounds__(kChooseThreads, RowLanes<T>::values * sizeof(T) <= 32 ? 2 : 1)
-choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
+// How the bounds of a page are spread over lanes that score it: chunk i of lane l is l + i * lanes, of the low and of the high ones.
+template <typename T> struct ScoreLanes {
+  static constexpr int chunks = kDim * static_cast<int>(sizeof(T)) / 16;
+  static constexpr int lanes = chunks % 16 == 0 ? 16 : RowLanes<T>::lanes;
+  static constexpr int per_lane = chunks / lanes;
+  static constexpr int values = per_lane * Vec<T>::n;
+  // pages of a team in flight: a power of two, and no more than its lanes, one of which each page's sum ends in
+  static constexpr int wished = per_lane == 1 ? 4 : (per_lane == 2 ? 2 : 1);
+  static constexpr int ahead = wished < lanes ? wished : lanes;
+  static_assert(lanes % ahead == 0 && lanes * per_lane == chunks);
+  static constexpr int at_once = 32 / lanes * ahead;                            // pages of a warp
+};
+
+// Single tokens, scores: a.cluster CTAs per (row, kv head) share out its pages, warp by warp; a team of lanes holds U and D in
+// registers and reads a page's bounds 16 bytes a lane, the next pages' ones before these are summed.  Scores are summed in 64 bits
+// and rounded once: the products of bfloat16 numbers are exact there, so neither the order of the sum nor its spread over lanes moves
+// a page across the border.  What bounds it is the reading of the bounds.
+template <typename T> __global__ void __launch_bounds__(kChooseThreads, ScoreLanes<T>::values <= 8 ? 2 : 1)
+score_pages_kernel(const __grid_constant__ ChooseArgs a) {
   using L = Vec<T>;
-  using R = RowLanes<T>;
-  extern __shared__ uint32_t keys[];
-  __shared__ double up[kDim], down[kDim];
-  __shared__ uint32_t scratch[select_words(kChooseWarps)];
-  if (a.cluster > 1) cluster_arrive();
-  pdl_trigger();
+  using R = ScoreLanes<T>;
+  constexpr int A = R::ahead;
+  pdl_launch_dependents();       // the choice comes next, and does nothing before its wait
   pdl_wait();
-  const int rank = blockIdx.x % a.cluster, unit = blockIdx.x / a.cluster, t = threadIdx.x;
+  const int share = blockIdx.x % a.cluster, unit = blockIdx.x / a.cluster, lane = threadIdx.x & 31;
   const int row = unit / a.kv_heads, head = unit % a.kv_heads;
   const int entry = a.token_entry[row], seen = visible_pages(a, a.positions[row], entry);
-  const int group = a.q_heads / a.kv_heads;
-  const int* table = a.block_table + static_cast<size_t>(seen > 0 ? entry : 0) * a.table_width;
-  for (int c = t; c < kDim; c += kChooseThreads)
-    parts_of(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim + c, group, up[c], down[c]);
-  __syncthreads();
-  constexpr int kTeams = kChooseThreads / R::lanes, kAhead = R::values <= 16 ? 2 : 1;
-  const int team = t / R::lanes, part = t % R::lanes, stride = a.cluster * kTeams;
-  double u[R::values], d[R::values];
+  const int from = (share * kChooseWarps + (threadIdx.x >> 5)) * R::at_once, stride = a.cluster * kChooseWarps * R::at_once;
+  if (seen <= a.budget || from >= seen) return;      // nothing to choose from, or nothing left of it
+  const int* table = a.block_table + static_cast<size_t>(entry) * a.table_width;
+  const int team = lane / R::lanes, part = lane % R::lanes;
+  // page j of the team in a round is from + team * A + j; ids are asked for a round before the bounds that they lead to
+  int ids[A];
 #pragma unroll
-  for (int i = 0; i < R::values; ++i) {
-    const int c = (part + i / L::n * R::lanes) * L::n + i % L::n;
-    u[i] = up[c], d[i] = down[c];
-  }
-  const uint32_t keys_at = a.cluster > 1 ? in_cluster(shared_address(keys), 0) : 0;
-  if (a.cluster > 1) cluster_wait();          // every CTA of the cluster has started
-  // the trip count is the same for all threads: the teams of a warp exchange sums
-  for (int base = rank * kTeams; base < seen; base += kAhead * stride) {
-    typename L::type low[kAhead][R::per_lane], high[kAhead][R::per_lane];
-    bool is[kAhead];
+  for (int j = 0; j < A; ++j) ids[j] = from + team * A + j < seen ? table[from + team * A + j] : -1;
+  typename L::type low[A][R::per_lane], high[A][R::per_lane];
+  bool is[A];
+  auto fetch = [&]() {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int p = base + j * stride + team, id = p < seen ? table[p] : -1;
-      is[j] = id >= 0 && id < a.num_pages;
+    for (int j = 0; j < A; ++j) {
+      is[j] = is_held(a, ids[j]);
       const typename L::type* at = reinterpret_cast<const typename L::type*>(
-          static_cast<const T*>(a.bounds) + (static_cast<size_t>(is[j] ? id : 0) * a.kv_heads + head) * 2 * kDim);
+          static_cast<const T*>(a.bounds) + (static_cast<size_t>(is[j] ? ids[j] : 0) * a.kv_heads + head) * 2 * kDim);
 #pragma unroll
-      for (int i = 0; i < R::per_lane; ++i) {
-        if (is[j]) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
-        else low[j][i] = high[j][i] = typename L::type{};
-      }
+      for (int i = 0; i < R::per_lane; ++i) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
     }
+  };
+  double u[R::values], d[R::values];
+  const int group = a.q_heads / a.kv_heads;
+  const typename L::type* q = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim);
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      double sum = 0, other = 0;
+  for (int i = 0; i < R::values; ++i) u[i] = d[i] = 0;
+  for (int h = 0; h < group; ++h) {
+#pragma unroll
+    for (int i = 0; i < R::per_lane; ++i) {
+      float v[L::n];
+      L::unpack(q[h * R::chunks + part + i * R::lanes], v);
+#pragma unroll
+      for (int x = 0; x < L::n; ++x) add_part(v[x], u[i * L::n + x], d[i * L::n + x]);
+    }
+  }
+  uint32_t* keys = a.keys + static_cast<size_t>(unit) * a.table_width;
+  fetch();
+  // the trip count is the same for all lanes: they exchange sums
+  for (int base = from; base < seen; base += stride) {
+    double sum[A];
+    uint32_t held = 0;
+#pragma unroll
+    for (int j = 0; j < A; ++j) {
+      if (is[j]) held |= 1u << j;
+      double other = 0;
+      sum[j] = 0;
 #pragma unroll
       for (int i = 0; i < R::per_lane; ++i) {
         float lo[L::n], hi[L::n];
@@ -271,31 +317,49 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
         L::unpack(high[j][i], hi);
 #pragma unroll
         for (int x = 0; x < L::n; ++x) {
-          sum = fma(static_cast<double>(hi[x]), u[i * L::n + x], sum);
+          sum[j] = fma(static_cast<double>(hi[x]), u[i * L::n + x], sum[j]);
           other = fma(static_cast<double>(lo[x]), d[i * L::n + x], other);
         }
       }
-      sum += other;
+      sum[j] += other;
+    }
+    const int next = base + stride + team * A;
 #pragma unroll
-      for (int o = 1; o < R::lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const int p = base + j * stride + team;
-      if (part == 0 && p < seen) {
-        const uint32_t key = !is[j] ? kKeyNone : (p < a.first || p >= seen - a.last ? kKeyAlways : score_key(sum));
-        if (a.cluster > 1) store_in_cluster(keys_at + p * 4, key); else keys[p] = key;
+    for (int j = 0; j < A; ++j) ids[j] = next + j < seen ? table[next + j] : -1;
+    // halves of the team add up halves of its pages, until every lane is left with one page (its place among the team's A: `mine`)
+    int mine = 0, width = R::lanes / 2;
+#pragma unroll
+    for (int n = A; n > 1; n /= 2, width /= 2) {
+      const bool upper = part & width;
+#pragma unroll
+      for (int j = 0; j < n / 2; ++j) {
+        const double give = upper ? sum[j] : sum[j + n / 2], keep = upper ? sum[j + n / 2] : sum[j];
+        sum[j] = keep + __shfl_xor_sync(0xffffffffu, give, width);
       }
+      mine += upper ? n / 2 : 0;
     }
+#pragma unroll
+    for (; width >= 1; width /= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], width);
+    fetch();
+    const int p = base + team * A + mine;
+    if (part % (R::lanes / A) == 0 && p < seen) keys[p] = key_of(a, p, seen, held >> mine & 1, sum[0]);
   }
-  if (a.cluster > 1) {
-    cluster_arrive();
-    if (rank != 0) {        // the first CTA is still there: it leaves after this barrier only
-      cluster_wait();
-      return;
-    }
-    cluster_wait();
-  } else {
-    __syncthreads();
-  }
-  select_pages<kChooseWarps>(keys, seen, a.budget, a.chosen + static_cast<size_t>(unit) * a.budget, scratch, t);
+}
+
+// Single tokens, choice: a CTA per (row, kv head).
+constexpr int kSelectWarps = 16;
+__global__ void __launch_bounds__(kSelectWarps * 32) select_pages_kernel(const __grid_constant__ ChooseArgs a) {
+  extern __shared__ uint32_t keys[];
+  __shared__ uint32_t scratch[select_words(kSelectWarps)];
+  pdl_trigger();
+  pdl_wait();
+  const int unit = blockIdx.x, row = unit / a.kv_heads, t = threadIdx.x;
+  const int entry = a.token_entry[row], seen = visible_pages(a, a.positions[row], entry);
+  const int* table = a.block_table + static_cast<size_t>(seen > 0 ? entry : 0) * a.table_width;
+  const uint32_t* made = a.keys + static_cast<size_t>(unit) * a.table_width;
+  for (int p = t; p < seen; p += kSelectWarps * 32) keys[p] = seen > a.budget ? made[p] : (is_held(a, table[p]) ? kKeyAlways : kKeyNone);
+  __syncthreads();
+  select_pages<kSelectWarps>(keys, seen, a.budget, a.chosen + static_cast<size_t>(unit) * a.budget, scratch, t);
 }
 
 // Rows of prompts: a cluster per (eight rows, kv head), the scores as a product [8 rows, 2 d] x [2 d, pages] on the 64-bit tensor
@@ -304,6 +368,10 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
 // The CTAs of the cluster share out the pages, then the rows: one warp chooses for a row.  Rows of several entries in one tile are
 // scored entry by entry.
 constexpr int kTileRows = 8;
+
+__device__ __forceinline__ void store_in_cluster(uint32_t address, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(address), "r"(v) : "memory");
+}
 
 __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
   asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};\n" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
@@ -344,6 +412,7 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads, 2) choos
     int r1 = r0, most = 0;
     while (r1 < here && entries[r1] == entry) most = max(most, seens[r1++]);
     const int* table = a.block_table + static_cast<size_t>(most > 0 ? entry : 0) * a.table_width;
+    const int steps = most > a.budget ? kSteps : 0;      // no row of these has anything to choose from: which pages are held is enough
     for (int p0 = (rank * kChooseWarps + warp) * 16; p0 < most; p0 += a.cluster * kChooseWarps * 16) {
       int id[2];
       const typename L::type* at[2];
@@ -356,7 +425,7 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads, 2) choos
         at[j] = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.bounds) + (static_cast<size_t>(max(id[j], 0)) * a.kv_heads + head) * 2 * kDim) + (lane & 3);
       }
 #pragma unroll 4
-      for (int step = 0; step < kSteps; ++step) {
+      for (int step = 0; step < steps; ++step) {
         float b[2][L::n];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -378,7 +447,7 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads, 2) choos
         for (int x = 0; x < 2; ++x) {
           const int of = __shfl_sync(0xffffffffu, id[j], (2 * (lane & 3) + x) * 4), p = p0 + 8 * j + 2 * (lane & 3) + x;
           if (r >= r0 && r < r1 && p < seen) {
-            const uint32_t key = of < 0 ? kKeyNone : (p < a.first || p >= seen - a.last ? kKeyAlways : score_key(c[j][x]));
+            const uint32_t key = key_of(a, p, seen, of >= 0, c[j][x]);
             const uint32_t place = (static_cast<uint32_t>(r % share) * a.table_width + p) * 4;
             if (a.cluster > 1) store_in_cluster(in_cluster(keys_at + place, r / share), key);
             else keys[place / 4] = key;
@@ -388,11 +457,10 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads, 2) choos
     }
     r0 = r1;
   }
+  __syncthreads();
   if (a.cluster > 1) {
     cluster_arrive();
     cluster_wait();
-  } else {
-    __syncthreads();
   }
   const int r = rank * share + warp;
   if (warp < share && r < here)
@@ -408,16 +476,28 @@ template <typename T> int launch_bounds_kernel(const BoundsArgs& a, int max_full
 
 constexpr int kChooseSharedBytes = 200 * 1024;
 
-// tile: eight rows to a cluster
-template <typename T> int launch_choose(const ChooseArgs& a, int tile, cudaStream_t stream) {
-  static DeviceOnce once, once_tile;
-  const long long units = static_cast<long long>(tile ? (a.rows + kTileRows - 1) / kTileRows : a.rows) * a.kv_heads;
-  const long long words = static_cast<long long>(a.table_width) * (tile ? kTileRows / a.cluster : 1);
-  const long long bytes = words * 4 + (tile ? 2 * kDim * kTileRows * 8 : 0);
+inline bool fits(const ChooseArgs& a) {
+  return a.table_width > 0 && a.entries > 0 && a.kv_heads > 0 && a.q_heads > 0 && a.q_heads % a.kv_heads == 0 && a.page_size > 0 &&
+         a.num_pages > 0 && a.first >= 0 && a.last >= 1 && a.budget >= a.first + a.last;
+}
+
+template <typename T> int launch_choose(const ChooseArgs& a, cudaStream_t stream) {
+  static DeviceOnce once;
+  const long long units = static_cast<long long>(a.rows) * a.kv_heads, bytes = static_cast<long long>(a.table_width) * 4;
   if (bytes > kChooseSharedBytes || units * a.cluster > 0x7fffffffll) return B200_ERR_TOO_LARGE;
-  const auto kernel = tile ? choose_tile_kernel<T> : choose_pages_kernel<T>;
-  if (const int status = configure_once(tile ? once_tile : once, kernel, kChooseSharedBytes)) return status;
-  launch_clusters(kernel, dim3(static_cast<unsigned>(units * a.cluster)), dim3(kChooseThreads), static_cast<size_t>(bytes), a.cluster, stream, a);
+  if (const int status = configure_once(once, select_pages_kernel, kChooseSharedBytes)) return status;
+  launch(score_pages_kernel<T>, dim3(static_cast<unsigned>(units * a.cluster)), dim3(kChooseThreads), 0, stream, a);
+  launch(select_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kSelectWarps * 32), static_cast<size_t>(bytes), stream, a);
+  return launch_status();
+}
+
+template <typename T> int launch_choose_tiles(const ChooseArgs& a, cudaStream_t stream) {
+  static DeviceOnce once;
+  const long long ctas = static_cast<long long>((a.rows + kTileRows - 1) / kTileRows) * a.kv_heads * a.cluster;
+  const long long bytes = static_cast<long long>(a.table_width) * (kTileRows / a.cluster) * 4 + 2 * kDim * kTileRows * 8;
+  if (bytes > kChooseSharedBytes || ctas > 0x7fffffffll) return B200_ERR_TOO_LARGE;
+  if (const int status = configure_once(once, choose_tile_kernel<T>, kChooseSharedBytes)) return status;
+  launch_clusters(choose_tile_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(kChooseThreads), static_cast<size_t>(bytes), a.cluster, stream, a);
   return launch_status();
 }
 
@@ -437,14 +517,28 @@ extern "C" int b200_page_bounds(const void* keys, void* bounds, const int* block
   return 0;
 }
 
+// keys: scratch of rows * kv_heads * table_width words, shares: CTAs that share out a row's pages.
 extern "C" int b200_choose_pages(const void* q, const void* bounds, const int* positions, const int* token_entry,
-                                 const int* block_table, int table_width, int* chosen, int rows, int entries, int q_heads, int kv_heads,
-                                 int page_size, int num_pages, int budget, int first, int last, int tile, int cluster, int dtype, cudaStream_t stream) {
+                                 const int* block_table, int table_width, int* chosen, uint32_t* keys, int rows, int entries, int q_heads,
+                                 int kv_heads, int page_size, int num_pages, int budget, int first, int last, int shares, int dtype,
+                                 cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (table_width <= 0 || entries <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || page_size <= 0 || num_pages <= 0 ||
-      first < 0 || last < 1 || budget < first + last || (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8)) return B200_ERR_BAD_SIZE;
-  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, table_width, rows, entries, q_heads, kv_heads, page_size,
+  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, keys, table_width, rows, entries, q_heads, kv_heads, page_size,
+               num_pages, budget, first, last, shares};
+  if (!fits(a) || shares < 1) return B200_ERR_BAD_SIZE;
+  B200_DISPATCH_DTYPE(dtype, T, return launch_choose<T>(a, stream));
+  return 0;
+}
+
+// The same for rows of prompts, eight to a cluster of `cluster` CTAs (1, 2, 4 or 8).
+extern "C" int b200_choose_pages_tiles(const void* q, const void* bounds, const int* positions, const int* token_entry,
+                                       const int* block_table, int table_width, int* chosen, int rows, int entries, int q_heads,
+                                       int kv_heads, int page_size, int num_pages, int budget, int first, int last, int cluster, int dtype,
+                                       cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, nullptr, table_width, rows, entries, q_heads, kv_heads, page_size,
                num_pages, budget, first, last, cluster};
-  B200_DISPATCH_DTYPE(dtype, T, return launch_choose<T>(a, tile, stream));
+  if (!fits(a) || (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8)) return B200_ERR_BAD_SIZE;
+  B200_DISPATCH_DTYPE(dtype, T, return launch_choose_tiles<T>(a, stream));
   return 0;
 }

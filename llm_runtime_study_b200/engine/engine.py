@@ -65,10 +65,16 @@ class Engine:
         every floating tensor must be stored in config.json's ``torch_dtype``),
         ``device_sampling`` (on by default: tokens are drawn on the device and a
         request's position, pending token and random counter live in its slot record
-        there; off: logits come back to the host for every step)."""
+        there; off: logits come back to the host for every step), ``attention_pages`` (off
+        by default: every token attends to all tokens before it; a number of at least 3: in
+        layers without a window every token, of prompts too, reads at most so many pages of
+        keys and values, the first page, the last two and those that can matter most to it
+        by the bounds of their keys)."""
 
         started = time.perf_counter()
-        loaded = load(model_dir, device=device, dtype=dtype, strict_dtype=options.get("strict_dtype", True))
+        attention_pages = options.pop("attention_pages", None)
+        loaded = load(model_dir, device=device, dtype=dtype, strict_dtype=options.get("strict_dtype", True),
+                      attention_pages=attention_pages)
         tokenizer = None
         if (Path(model_dir) / "tokenizer.json").is_file():
             from ..tokenizer import load_tokenizer
@@ -87,10 +93,12 @@ class Engine:
         max_batch_size: int = 1, use_cuda_graph: bool = True, on_device: bool = True, **options: Any,
     ) -> "Engine":
         """A model of the given ``config.json`` object with seeded random weights
-        (linear and embedding N(0, 0.02), norm weights 1 + N(0, 0.05))."""
+        (linear and embedding N(0, 0.02), norm weights 1 + N(0, 0.05)); the options of
+        ``from_model_dir`` apply."""
 
         started = time.perf_counter()
-        loaded = load_random(config, seed, device=device, dtype=dtype, on_device=on_device)
+        loaded = load_random(config, seed, device=device, dtype=dtype, on_device=on_device,
+                             attention_pages=options.pop("attention_pages", None))
         engine = cls(loaded=loaded, max_seq_len=max_seq_len, max_batch_size=max_batch_size,
                      use_cuda_graph=use_cuda_graph, source=("random", dict(config), seed, on_device), **options)
         engine.synchronize()
@@ -105,6 +113,12 @@ class Engine:
     @property
     def dtype(self) -> torch.dtype:
         return self.loaded.runtime.dtype
+
+    @property
+    def attention_pages(self) -> int | None:
+        """The most pages of keys and values a token reads in layers without a window (``None``: all)."""
+
+        return self.loaded.runtime.attention_pages
 
     @property
     def model(self):
@@ -185,10 +199,12 @@ class Engine:
         if self.source is None:
             raise EngineError("this engine does not know where its weights came from and cannot be moved")
         if self.source[0] == "dir":
-            self.loaded = load(self.source[1], device=new_device, dtype=new_dtype, strict_dtype=self.strict_dtype)
+            self.loaded = load(self.source[1], device=new_device, dtype=new_dtype, strict_dtype=self.strict_dtype,
+                               attention_pages=self.attention_pages)
         else:
             _, config, seed, on_device = self.source
-            self.loaded = load_random(config, seed, device=new_device, dtype=new_dtype, on_device=on_device)
+            self.loaded = load_random(config, seed, device=new_device, dtype=new_dtype, on_device=on_device,
+                                      attention_pages=self.attention_pages)
         self._runner = None
         self._sampler = None
         self.synchronize()

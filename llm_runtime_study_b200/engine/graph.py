@@ -20,9 +20,11 @@ launch in the graph, how many of its grid's parts this batch's longest sequence 
 (``ops/attention_bf16.LiveParts``); the CTAs of the other parts leave at once.
 
 All per-step input lives in one persistent device buffer whose layout is fixed by the
-bucket and the table width: the slots of the batch, the numbers of parts, the block tables.  It is copied
-only when it differs from what the device already holds, so a replay is at most one
-host-to-device copy plus one graph launch.  Graphs share one memory pool: they run one
+bucket and the table width: the slots of the batch and the numbers of parts.  It is copied
+only when it differs from what the device already holds.  The block tables are made in the step from
+the tables of all slots (``cache/tables.py``), into which the pages taken since the last
+step are put before the replay; so a step in which no request took a page is at most one
+host-to-device copy plus one graph launch, however long the sequences are.  Graphs share one memory pool: they run one
 after the other on one stream, and what leaves a graph (the drawn ids) lies outside it.
 Steps that hold prompt portions run eagerly.
 """
@@ -54,14 +56,14 @@ class DecodeGraph:
         self.table_widths = [_round_up(-(-manager.max_seq_len // pool.page_size), 4) for pool in manager.groups]
         self.groups = len(manager.layout.groups)
         b = batch
-        # what the host sends every step (slots, numbers of parts, tables), then what never changes, then what the device fills in
-        sizes = [b, LIVE_PLACES] + [b * w for w in self.table_widths] + [b, b + 1, b] + [b, b, b]
+        # what the host sends every step (slots, numbers of parts), then what never changes, then what the device fills in
+        sizes = [b, LIVE_PLACES] + [b, b + 1, b, b] + [b, b, b] + [b * w for w in self.table_widths]
         self.offsets, total = [], 0
         for size in sizes:
             self.offsets.append(total)
             total += _round_up(size, 4)
         self.sizes = sizes
-        self.sent = self.offsets[2 + self.groups]          # words copied per step
+        self.sent = self.offsets[2]                        # words copied per step
         device = runner.runtime.device
         self.dev = torch.zeros(total, dtype=torch.int32, device=device)
         self.host = [torch.zeros(self.sent, dtype=torch.int32, pin_memory=True) for _ in range(2)]
@@ -73,26 +75,26 @@ class DecodeGraph:
         self.logits: torch.Tensor | None = None
         self.kernel_launches = 0
         ramp = torch.arange(b + 1, dtype=torch.int32, device=device)
-        g = self.groups
-        self._view(2 + g).copy_(ramp[:b])                   # token -> entry
-        self._view(3 + g).copy_(ramp)                       # first token of each entry
-        self._view(4 + g).copy_(ramp[:b])                   # rows whose logits are wanted: all
+        self._view(2).copy_(ramp[:b])                       # token -> entry
+        self._view(3).copy_(ramp)                           # first token of each entry
+        self._view(4).copy_(ramp[:b])                       # rows whose logits are wanted: all
+        self._view(5).fill_(1)                              # new tokens of each entry
         self.ctx = self._static_context()
 
     def _view(self, i: int) -> torch.Tensor:
         return self.dev[self.offsets[i] : self.offsets[i] + self.sizes[i]]
 
     def _static_context(self) -> StepContext:
-        runner, b, g = self.runner, self.batch, self.groups
+        runner, b = self.runner, self.batch
         ctx = StepContext(runner.runtime, runner.manager)
         ctx.num_tokens = ctx.num_entries = ctx.num_logit_rows = b
         from ..ops.attention_bf16 import LiveParts
 
         ctx.slots = ctx.row_slots = self._view(0)
         ctx.live_parts = LiveParts(self._view(1), self.bound)
-        ctx.tables = [self._view(2 + i).view(b, self.table_widths[i]) for i in range(g)]
-        ctx.token_entry, ctx.q_start, ctx.logit_rows = self._view(2 + g), self._view(3 + g), self._view(4 + g)
-        ctx.token_ids, ctx.positions, ctx.kv_len = self._view(5 + g), self._view(6 + g), self._view(7 + g)
+        ctx.token_entry, ctx.q_start, ctx.logit_rows, ctx.counts = (self._view(i) for i in range(2, 6))
+        ctx.token_ids, ctx.positions, ctx.kv_len = (self._view(i) for i in range(6, 9))
+        ctx.tables = [self._view(9 + i).view(b, self.table_widths[i]) for i in range(self.groups)]
         ctx.q_lens = [1] * b
         # kernels launched under capture may only size their grids from limits that never change
         ctx.kv_lens = [self.bound] * b
@@ -103,23 +105,20 @@ class DecodeGraph:
         return ctx
 
     def _fill(self, requests: Sequence[RequestCache]) -> None:
-        """This step's slots and block tables.  Rows beyond the requests are padding: the
-        slot that is never live and an empty block table."""
+        """This step's slots, and the pages its requests have taken.  Rows beyond the requests are padding: the
+        slot that is never live, and so an empty row of the block table."""
 
         b = self.batch
-        manager = self.runner.manager
-        sent = np.full(self.sent, -1, dtype=np.int32)
+        runner, manager = self.runner, self.runner.manager
+        if manager.tables is not None:
+            changes = manager.tables.changes(requests)
+            if any(cells.shape[1] for cells in changes):
+                runner.set_tables(requests, changes, runner._send(changes))
+        sent = np.zeros(self.sent, dtype=np.int32)
         sent[:b] = manager.padding_slot
         sent[: len(requests)] = [r.slot for r in requests]
-        sent[b : self.offsets[2]] = 0
         parts = self.ctx.live_parts.fill(max(r.length for r in requests) + 1)    # for the longest sequence once this step has run
         sent[self.offsets[1] : self.offsets[1] + len(parts)] = parts
-        for g in range(self.groups):
-            o, w = self.offsets[2 + g], self.table_widths[g]
-            table = sent[o : o + b * w].reshape(b, w)
-            for i, r in enumerate(requests):
-                row = r.tables[g]
-                table[i, : len(row)] = row
         if self.on_device is not None and not self.always_send and np.array_equal(sent, self.on_device):
             return
         self.turn ^= 1
@@ -134,13 +133,10 @@ class DecodeGraph:
         self.on_device = sent
 
     def _launches(self, sampler: Any, ids: torch.Tensor) -> torch.Tensor:
-        from ..ops import slots as slot_ops
-
-        records = self.runner.manager.slots.records
         ctx = self.ctx
-        slot_ops.slot_load(records, ctx.slots, ctx.token_ids, ctx.positions, ctx.kv_len)
+        self.runner.load_decode_maps(ctx)
         logits = self.runner.model.forward(ctx)
-        sampler.sample_slots(logits, records, ctx.row_slots, ids, filtered=self.filtered)
+        sampler.sample_slots(logits, self.runner.manager.slots.records, ctx.row_slots, ids, filtered=self.filtered)
         return logits
 
     def capture(self, sampler: Any, ids: torch.Tensor, pool: Any) -> None:

@@ -12,6 +12,8 @@ from ..cache.manager import CacheManager
 from ..errors import EngineError
 from ..models.loading import load_model_dir, random_model
 from ..models.model import DecoderModel
+from ..ops import sparse_pages
+from ..parts.attention import FIRST_PAGES, LAST_PAGES
 from ..parts.base import Runtime
 from .step import StepRunner
 
@@ -78,24 +80,50 @@ class LoadedModel:
             max_requests=max_requests, dtype=self.runtime.dtype, device=self.runtime.device,
             max_seq_len=max_seq_len or description.max_positions, max_step_tokens=max_step_tokens,
         )
+        if self.runtime.attention_pages is not None:
+            for pool in manager.groups:
+                if pool.group.requirement.page_tensors and pool.pages_for(manager.max_seq_len) > sparse_pages.MAX_TABLE_WIDTH:
+                    raise EngineError(f"attention_pages takes sequences of at most {sparse_pages.MAX_TABLE_WIDTH} pages; "
+                                      f"{manager.max_seq_len} tokens are {pool.pages_for(manager.max_seq_len)} pages of {pool.page_size}")
         return StepRunner(
             self.model, manager, self.runtime, vocab_size=description.vocab_size,
             max_positions=description.max_positions,
         )
 
 
-def load(model_dir: str | Path, *, device="auto", dtype="auto", strict_dtype: bool = True) -> LoadedModel:
+def resolve_attention_pages(requested: int | None) -> int | None:
+    if requested is None:
+        return None
+    least = FIRST_PAGES + LAST_PAGES
+    if isinstance(requested, bool) or not isinstance(requested, int) or requested < least:
+        raise EngineError(f"attention_pages must be None or a whole number of at least {least}, got {requested!r}")
+    return requested
+
+
+def _check_attention_pages(loaded: LoadedModel) -> LoadedModel:
+    if loaded.runtime.attention_pages is not None:
+        groups = loaded.model.cache_layout().groups
+        if not any(name == "bounds" for group in groups for name, _ in group.requirement.page_tensors):
+            raise EngineError("attention_pages was given, but no layer of this model chooses pages (kind gqa_attention without a window)")
+    return loaded
+
+
+def load(model_dir: str | Path, *, device="auto", dtype="auto", strict_dtype: bool = True,
+         attention_pages: int | None = None) -> LoadedModel:
     from ..config.registry import load_config
 
     load_config(model_dir)  # a bad folder or config.json is reported before anything about the device
-    runtime = Runtime(resolve_device(device), resolve_dtype(dtype))
+    attention_pages = resolve_attention_pages(attention_pages)
+    runtime = Runtime(resolve_device(device), resolve_dtype(dtype), attention_pages)
     with torch.cuda.device(runtime.device):
         model, config, _ = load_model_dir(model_dir, runtime, strict_dtype=strict_dtype)
-    return LoadedModel(model, config, runtime)
+    return _check_attention_pages(LoadedModel(model, config, runtime))
 
 
-def load_random(config_dict: Mapping[str, Any], seed: int, *, device="auto", dtype="auto", on_device=False) -> LoadedModel:
-    runtime = Runtime(resolve_device(device), resolve_dtype(dtype))
+def load_random(config_dict: Mapping[str, Any], seed: int, *, device="auto", dtype="auto", on_device=False,
+                attention_pages: int | None = None) -> LoadedModel:
+    attention_pages = resolve_attention_pages(attention_pages)
+    runtime = Runtime(resolve_device(device), resolve_dtype(dtype), attention_pages)
     with torch.cuda.device(runtime.device):
         model, config, weights = random_model(config_dict, seed, runtime, on_device=on_device)
-    return LoadedModel(model, config, runtime, weights)
+    return _check_attention_pages(LoadedModel(model, config, runtime, weights))

@@ -25,6 +25,7 @@ from ..cache.manager import CacheManager, RequestCache
 from ..cache.slots import SLOT_WORDS, SlotRecord
 from ..errors import GenerationError, KVCacheError, SamplingError
 from ..ops import attention as attention_ops
+from ..ops import page_tables
 from ..parts.base import Runtime
 
 
@@ -75,7 +76,9 @@ class StepContext:
         self.kv_len: torch.Tensor = None         # [R] int32 length of each request after this step
         self.slots: torch.Tensor = None          # [R] int32 request slot of each entry
         self.logit_rows: torch.Tensor = None     # [M] int32 rows whose logits are wanted
+        self.counts: torch.Tensor = None         # [R] int32 new tokens of each entry
         self.tables: list[torch.Tensor] = []     # per page group: [R, width] int32
+        self._slot_maps: dict[int, torch.Tensor] = {}
         # host-side copies, for choosing kernels and grids
         self.q_lens: list[int] = []
         self.kv_lens: list[int] = []
@@ -91,6 +94,22 @@ class StepContext:
 
     def block_table(self, group: int) -> torch.Tensor:
         return self.tables[group]
+
+    def slot_map(self, group: int) -> torch.Tensor:
+        """[N] int64: where each token of the step lies in a group's pages, as a row of ``[pages * page_size]`` (-1: a row that
+        pads the batch), for parts that write their pages with tensor operations.  On a CUDA device."""
+
+        made = self._slot_maps.get(group)
+        if made is None:
+            tables = self.tables[group]
+            made = torch.empty(self.num_tokens, dtype=torch.int64, device=tables.device)
+            out = page_tables.StepMaps(torch.empty_like(tables), slot_map=made)
+            rows = torch.arange(tables.shape[0], dtype=torch.int32, device=tables.device)
+            page_tables.step_maps(tables, slots=rows, kv_len=self.kv_len, counts=self.counts, page_size=self.manager.groups[group].page_size,
+                                  num_tokens=self.num_tokens, out=out)
+            if not self.captured:       # a captured step's map belongs to the graph: every replay makes it anew
+                self._slot_maps[group] = made
+        return made
 
     def attention(self, q: torch.Tensor, cache: Any, *, scale: float, window: int = 0) -> torch.Tensor:
         return attention_ops.paged_attention(q, cache, self, scale=scale, window=window)
@@ -221,29 +240,58 @@ class StepRunner:
             manager.grow(entry.request, start + n)
         return q_lens, starts
 
+    def _send(self, pieces: Sequence[np.ndarray]) -> list[torch.Tensor]:
+        """The int32 pieces on the device, in one copy; each starts on a 16-byte boundary."""
+
+        offsets, total = [], 0
+        for piece in pieces:
+            offsets.append(total)
+            total += _round_up(piece.size, 4)
+        packed = np.zeros(total, dtype=np.int32)
+        for piece, off in zip(pieces, offsets):
+            packed[off : off + piece.size] = piece.reshape(-1)
+        dev = self._buffers.upload(packed)
+        return [dev[off : off + piece.size].view(piece.shape) for piece, off in zip(pieces, offsets)]
+
+    def _host_tables(self, requests: Sequence[RequestCache], table_width: int | None = None) -> list[np.ndarray]:
+        """Block tables put together on the host: for a device that runs no kernels."""
+
+        tables = []
+        for g in range(len(self.manager.layout.groups)):
+            width = max(len(r.tables[g]) for r in requests)
+            table = np.full((len(requests), table_width or _round_up(max(width, 1), 4)), -1, dtype=np.int32)
+            for i, r in enumerate(requests):
+                table[i, : len(r.tables[g])] = r.tables[g]
+            tables.append(table)
+        return tables
+
+    def set_tables(self, requests: Sequence[RequestCache], changes: Sequence[np.ndarray], sent: Sequence[torch.Tensor]) -> None:
+        """Put the cells of the requests' block tables that changed (``sent``: ``changes`` on the device) into the device's tables."""
+
+        device_tables = self.manager.tables
+        for table, cells in zip(device_tables.tensors, sent):
+            if cells.shape[1]:
+                page_tables.page_table_set(table, rows=cells[0], columns=cells[1], pages=cells[2])
+        device_tables.sent(requests)
+
+    def _empty_tables(self, requests: Sequence[RequestCache], table_width: int | None = None) -> list[torch.Tensor]:
+        """Room for the step's block tables, as wide as its longest request's."""
+
+        widths = [table_width or _round_up(max(max(len(r.tables[g]) for r in requests), 1), 4) for g in range(len(self.manager.groups))]
+        return [torch.empty((len(requests), w), dtype=torch.int32, device=self.runtime.device) for w in widths]
+
     def _pack_context(self, entries, q_lens, starts, table_width) -> StepContext:
         manager = self.manager
         num_tokens, num_entries = sum(q_lens), len(entries)
+        requests = [e.request for e in entries]
         token_ids = np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in entries])
-        positions = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, q_lens)])
-        token_entry = np.repeat(np.arange(num_entries, dtype=np.int32), q_lens)
         q_start = np.zeros(num_entries + 1, dtype=np.int32)
         np.cumsum(q_lens, out=q_start[1:])
         kv_lens = [s + n for s, n in zip(starts, q_lens)]
-        slots = np.asarray([e.request.slot for e in entries], dtype=np.int32)
+        slots = np.asarray([r.slot for r in requests], dtype=np.int32)
         logit_rows = np.asarray(
             [q_start[i] + int(w) for i, e in enumerate(entries) for w in e.want], dtype=np.int32
         )
-        tables = []
-        for g in range(len(manager.layout.groups)):
-            width = max(len(e.request.tables[g]) for e in entries)
-            width = table_width if table_width is not None else _round_up(max(width, 1), 4)
-            table = np.full((num_entries, width), -1, dtype=np.int32)
-            for i, e in enumerate(entries):
-                row = e.request.tables[g]
-                table[i, : len(row)] = row
-            tables.append(table)
-
         sampled = [e for e in entries if e.sample is not None]
         row_slots = np.asarray([e.request.slot for e in sampled], dtype=np.int32)
         staged = np.zeros((len(sampled), SLOT_WORDS), dtype=np.int32)
@@ -252,30 +300,32 @@ class StepRunner:
                 e.sample = replace(e.sample, position=length)
         for i, e in enumerate(sampled):
             staged[i] = manager.slots.note(e.request.slot, e.sample)
-        pieces = [token_ids, positions, token_entry, q_start, np.asarray(kv_lens, dtype=np.int32), slots,
-                  logit_rows, *[t.reshape(-1) for t in tables], row_slots, staged.reshape(-1)]
-        # every piece starts on a 16-byte boundary
-        offsets, total = [], 0
-        for piece in pieces:
-            offsets.append(total)
-            total += _round_up(piece.shape[0], 4)
-        packed = np.zeros(total, dtype=np.int32)
-        for piece, off in zip(pieces, offsets):
-            packed[off : off + piece.shape[0]] = piece
-        dev = self._buffers.upload(packed)
-
-        def view(i: int) -> torch.Tensor:
-            return dev[offsets[i] : offsets[i] + pieces[i].shape[0]]
+        pieces = [token_ids, np.asarray(kv_lens, dtype=np.int32), np.asarray(q_lens, dtype=np.int32), slots, logit_rows, row_slots, staged]
 
         ctx = StepContext(self.runtime, manager)
         ctx.num_tokens, ctx.num_entries, ctx.num_logit_rows = num_tokens, num_entries, int(logit_rows.shape[0])
-        ctx.token_ids, ctx.positions, ctx.token_entry = view(0), view(1), view(2)
-        ctx.q_start, ctx.kv_len, ctx.slots, ctx.logit_rows = view(3), view(4), view(5), view(6)
-        ctx.tables = [view(7 + g).view(num_entries, tables[g].shape[1]) for g in range(len(tables))]
-        ctx.row_slots = view(7 + len(tables))
-        ctx.staged_records = view(8 + len(tables)).view(len(sampled), SLOT_WORDS)
+        if manager.tables is not None:
+            # the requests' tables are on the device already: what changed of them goes there, the rest is made there
+            changes = manager.tables.changes(requests)
+            sent = self._send([*pieces, *changes])
+            self.set_tables(requests, changes, sent[len(pieces) :])
+            tables = self._empty_tables(requests, table_width)
+            ints = [torch.empty(n, dtype=torch.int32, device=self.runtime.device) for n in (num_entries + 1, num_tokens, num_tokens)]
+            for g, table in enumerate(tables):
+                page_tables.step_maps(manager.tables.tensors[g], slots=sent[3], kv_len=sent[1], counts=sent[2],
+                                      page_size=manager.groups[g].page_size, num_tokens=num_tokens,
+                                      out=page_tables.StepMaps(table, *(ints if g == 0 else ())))
+            ctx.q_start, ctx.positions, ctx.token_entry = ints
+        else:
+            positions = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, q_lens)])
+            token_entry = np.repeat(np.arange(num_entries, dtype=np.int32), q_lens)
+            sent = self._send([*pieces, q_start, positions, token_entry, *self._host_tables(requests, table_width)])
+            ctx.q_start, ctx.positions, ctx.token_entry = sent[len(pieces) : len(pieces) + 3]
+            tables = sent[len(pieces) + 3 :]
+        ctx.token_ids, ctx.kv_len, ctx.counts, ctx.slots, ctx.logit_rows, ctx.row_slots, ctx.staged_records = sent[: len(pieces)]
+        ctx.tables = list(tables)
         ctx.q_lens, ctx.kv_lens = q_lens, kv_lens
-        ctx.entry_slots = [e.request.slot for e in entries]
+        ctx.entry_slots = [r.slot for r in requests]
         ctx.max_q_len, ctx.max_kv_len = max(q_lens), max(kv_lens)
         ctx.all_decode = ctx.max_q_len == 1
         ctx.logits_at_every_row = logit_rows.shape[0] == num_tokens and bool((logit_rows == np.arange(num_tokens)).all())
@@ -366,48 +416,50 @@ class StepRunner:
     def _decode_eager(self, requests: Sequence[RequestCache], sampler: Any, filtered: bool):
         """The launches a captured decode step holds, issued one by one."""
 
-        from ..ops import slots as slot_ops
-
         manager = self.manager
         n = len(requests)
         starts = [r.length for r in requests]
-        tables = []
-        for g in range(len(manager.layout.groups)):
-            width = _round_up(max(max(len(r.tables[g]) for r in requests), 1), 4)
-            table = np.full((n, width), -1, dtype=np.int32)
-            for i, r in enumerate(requests):
-                table[i, : len(r.tables[g])] = r.tables[g]
-            tables.append(table)
         ramp = np.arange(n + 1, dtype=np.int32)
         slots = np.asarray([r.slot for r in requests], dtype=np.int32)
         blank = np.zeros(n, dtype=np.int32)
         # token ids, positions and lengths are filled in on the device from the slot records
-        pieces = [blank, blank, ramp[:n], ramp, blank, slots, ramp[:n], *[t.reshape(-1) for t in tables]]
-        offsets, total = [], 0
-        for piece in pieces:
-            offsets.append(total)
-            total += _round_up(piece.shape[0], 4)
-        packed = np.zeros(total, dtype=np.int32)
-        for piece, off in zip(pieces, offsets):
-            packed[off : off + piece.shape[0]] = piece
-        dev = self._buffers.upload(packed)
-
-        def view(i: int) -> torch.Tensor:
-            return dev[offsets[i] : offsets[i] + pieces[i].shape[0]]
+        pieces = [blank, blank, blank, ramp, slots, np.ones(n, dtype=np.int32)]
+        changes = manager.tables.changes(requests) if manager.tables is not None else []
+        sent = self._send([*pieces, *changes])
 
         ctx = StepContext(self.runtime, manager)
         ctx.num_tokens = ctx.num_entries = ctx.num_logit_rows = n
-        ctx.token_ids, ctx.positions, ctx.token_entry = view(0), view(1), view(2)
-        ctx.q_start, ctx.kv_len, ctx.slots, ctx.logit_rows = view(3), view(4), view(5), view(6)
-        ctx.tables = [view(7 + g).view(n, tables[g].shape[1]) for g in range(len(tables))]
+        ctx.token_ids, ctx.positions, ctx.kv_len, ctx.q_start, ctx.slots, ctx.counts = sent[: len(pieces)]
+        ctx.token_entry = ctx.logit_rows = ctx.q_start[:n]
+        if changes:
+            self.set_tables(requests, changes, sent[len(pieces) :])
+            ctx.tables = self._empty_tables(requests)
         ctx.row_slots = ctx.slots
         ctx.q_lens, ctx.kv_lens = [1] * n, [s + 1 for s in starts]
         ctx.entry_slots = [r.slot for r in requests]
         ctx.max_q_len, ctx.max_kv_len = 1, max(ctx.kv_lens)
         ctx.all_decode = ctx.logits_at_every_row = True
         with torch.inference_mode():
-            slot_ops.slot_load(manager.slots.records, ctx.slots, ctx.token_ids, ctx.positions, ctx.kv_len)
+            self.load_decode_maps(ctx)
             logits = self.model.forward(ctx)
             sampler.sample_slots(logits, manager.slots.records, ctx.row_slots, self._ids_device, filtered=filtered)
         self.last_context = ctx
         return self._ids_device, logits
+
+    def load_decode_maps(self, ctx: StepContext) -> None:
+        """Fill a decode step's token ids, positions, lengths and block tables from the slot records and the requests' tables."""
+
+        from ..ops import slots as slot_ops
+
+        manager = self.manager
+        records = manager.slots.records
+        for g, table in enumerate(ctx.tables):
+            of, page_size = manager.tables.tensors[g], manager.groups[g].page_size
+            if g == 0:
+                page_tables.slot_load_maps(records, ctx.slots, ctx.token_ids, ctx.positions, ctx.kv_len, tables=of, page_size=page_size,
+                                           block_table=table)
+            else:
+                page_tables.step_maps(of, slots=ctx.slots, kv_len=ctx.kv_len, counts=ctx.counts, page_size=page_size,
+                                      num_tokens=ctx.num_tokens, out=page_tables.StepMaps(table))
+        if not ctx.tables:       # no layer keeps pages
+            slot_ops.slot_load(records, ctx.slots, ctx.token_ids, ctx.positions, ctx.kv_len)

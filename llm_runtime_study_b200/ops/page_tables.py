@@ -7,14 +7,16 @@ from dataclasses import dataclass
 import torch
 
 from . import native
+from ..cache.slots import SLOT_WORDS
 from ..errors import KernelError
-from .native import c_int, c_void_p, ptr, require
+from .native import c_int, c_void_p, pointer
 
 native.register_library(
     "b200_page_tables", ("page_tables.cu",),
     {
         "b200_page_table_set": [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
         "b200_step_maps": [c_void_p, c_int, c_int] + [c_void_p] * 4 + [c_int] + [c_void_p] * 4 + [c_int, c_int, c_int, c_void_p],
+        "b200_slot_load_maps": [c_void_p, c_int] + [c_void_p] * 5 + [c_int, c_int, c_void_p] + [c_int] * 3 + [c_void_p],
     },
 )
 
@@ -33,19 +35,15 @@ class StepMaps:
 def page_table_set(tables: torch.Tensor, *, rows: torch.Tensor, columns: torch.Tensor, pages: torch.Tensor) -> None:
     """``tables[rows[i], columns[i]] = pages[i]`` (all int32, the cells distinct); a cell outside the table is left out."""
 
-    native.require_here(tables, "tables")
-    require(tables, "tables", dtype=torch.int32, dims=2)
-    require(rows, "rows", dtype=torch.int32, dims=1)
-    for t, name in ((columns, "columns"), (pages, "pages")):
-        require(t, name, dtype=torch.int32, shape=rows.shape)
-    for t, name in ((rows, "rows"), (columns, "columns"), (pages, "pages")):
-        native.require_here(t, name)
-    if tables.numel() == 0:
+    at = pointer(tables, "tables", torch.int32, dims=2)
+    rows_at = pointer(rows, "rows", torch.int32, dims=1)
+    shape = rows.shape
+    columns_at, pages_at = pointer(columns, "columns", torch.int32, shape=shape), pointer(pages, "pages", torch.int32, shape=shape)
+    slots, width = tables.shape
+    if not slots or not width:
         raise KernelError(f"a page table of shape {tuple(tables.shape)} has no cells")
-    if rows.shape[0] == 0:
-        return
-    native.call("b200_page_table_set", ptr(tables), tables.shape[0], tables.shape[1], ptr(rows), ptr(columns), ptr(pages),
-                rows.shape[0], native.stream_ptr())
+    if shape[0]:
+        native.call("b200_page_table_set", at, slots, width, rows_at, columns_at, pages_at, shape[0], native.stream_ptr())
 
 
 def step_maps(
@@ -60,39 +58,51 @@ def step_maps(
     ``out``: tensors to write into, which may have room for more entries and tokens than there are (those are left as they are);
     what is ``None`` there is not made."""
 
-    native.require_here(tables, "tables")
-    require(tables, "tables", dtype=torch.int32, dims=2)
-    require(slots, "slots", dtype=torch.int32, dims=1)
+    at = pointer(tables, "tables", torch.int32, dims=2)
+    slots_at = pointer(slots, "slots", torch.int32, dims=1)
     entries = slots.shape[0]
-    for t, name in ((kv_len, "kv_len"), (counts, "counts")):
-        require(t, name, dtype=torch.int32, shape=(entries,))
-    if tables.numel() == 0 or page_size <= 0 or num_tokens < 0 or (width is not None and width <= 0):
+    kv_len_at, counts_at = pointer(kv_len, "kv_len", torch.int32, shape=(entries,)), pointer(counts, "counts", torch.int32, shape=(entries,))
+    table_rows, table_width = tables.shape
+    if not table_rows or not table_width or page_size <= 0 or num_tokens < 0 or (width is not None and width <= 0):
         raise KernelError(f"tables {tuple(tables.shape)}, page_size {page_size}, num_tokens {num_tokens} and width {width} do not fit")
     if out is None:
-        def ints(*shape, dtype=torch.int32):
-            return torch.empty(shape, dtype=dtype, device=tables.device)
-
-        out = StepMaps(ints(entries, tables.shape[1] if width is None else width), ints(entries + 1), ints(num_tokens),
-                       ints(num_tokens), ints(num_tokens, dtype=torch.int64))
-        if entries == 0:
-            out.q_start.zero_()
+        device = tables.device
+        # the three short ones in one piece of memory
+        q_start, positions, token_entry = torch.empty(entries + 1 + 2 * num_tokens, dtype=torch.int32, device=device).split_with_sizes(
+            (entries + 1, num_tokens, num_tokens))
+        out = StepMaps(torch.empty((entries, width or table_width), dtype=torch.int32, device=device), q_start, positions, token_entry,
+                       torch.empty(num_tokens, dtype=torch.int64, device=device))
+        if not entries:
+            q_start.zero_()
     elif width is not None and out.block_table.shape[-1] != width:
         raise KernelError(f"out.block_table has {out.block_table.shape[-1]} columns, not {width}")
-    require(out.block_table, "out.block_table", dtype=torch.int32, dims=2)
-    for t, name, least, dtype in ((out.block_table, "block_table", entries, torch.int32), (out.q_start, "q_start", entries + 1, torch.int32),
-                                  (out.positions, "positions", num_tokens, torch.int32),
-                                  (out.token_entry, "token_entry", num_tokens, torch.int32),
-                                  (out.slot_map, "slot_map", num_tokens, torch.int64)):
-        if t is None:
-            continue
-        require(t, f"out.{name}", dtype=dtype, dims=2 if t is out.block_table else 1)
-        if t.shape[0] < least:
-            raise KernelError(f"out.{name} has room for {t.shape[0]}, {least} are needed")
-    for t, name in ((slots, "slots"), (kv_len, "kv_len"), (counts, "counts"), (out.block_table, "out.block_table")):
-        native.require_here(t, name)
-    if entries == 0:
-        return out
-    native.call("b200_step_maps", ptr(tables), tables.shape[0], tables.shape[1], ptr(slots), ptr(kv_len), ptr(counts),
-                ptr(out.block_table), out.block_table.shape[1], ptr(out.q_start), ptr(out.positions), ptr(out.token_entry),
-                ptr(out.slot_map), entries, int(page_size), int(num_tokens), native.stream_ptr())
+    block_table = pointer(out.block_table, "out.block_table", torch.int32, dims=2)
+    rooms = [(out.q_start, "out.q_start", torch.int32, entries + 1), (out.positions, "out.positions", torch.int32, num_tokens),
+             (out.token_entry, "out.token_entry", torch.int32, num_tokens), (out.slot_map, "out.slot_map", torch.int64, num_tokens)]
+    pointers = [None if t is None else pointer(t, name, dtype, dims=1, align=dtype.itemsize) for t, name, dtype, _ in rooms]
+    for t, name, _, least in [(out.block_table, "out.block_table", None, entries), *rooms]:
+        if t is not None and t.shape[0] < least:
+            raise KernelError(f"{name} has room for {t.shape[0]}, {least} are needed")
+    if entries:
+        native.call("b200_step_maps", at, table_rows, table_width, slots_at, kv_len_at, counts_at, block_table, out.block_table.shape[1],
+                    *pointers, entries, int(page_size), int(num_tokens), native.stream_ptr())
     return out
+
+
+def slot_load_maps(records: torch.Tensor, slots: torch.Tensor, token_ids: torch.Tensor, positions: torch.Tensor, kv_len: torch.Tensor, *,
+                   tables: torch.Tensor, page_size: int, block_table: torch.Tensor) -> None:
+    """``slots.slot_load`` (a decode batch's token ids, positions and lengths from the records of its slots, whose positions
+    advance) and the batch's ``block_table`` from ``tables`` by those lengths, as ``step_maps`` makes it, in one launch.  The slots
+    of live records are distinct."""
+
+    at = pointer(records, "records", torch.int32, dims=2)
+    if records.shape[1] != SLOT_WORDS:
+        raise KernelError(f"records of {records.shape[1]} words are not slot records")
+    n = slots.shape[0]
+    given = [pointer(t, name, torch.int32, shape=(n,)) for t, name in ((slots, "slots"), (token_ids, "token_ids"), (positions, "positions"),
+                                                                     (kv_len, "kv_len"))]
+    tables_at, block_at = pointer(tables, "tables", torch.int32, dims=2), pointer(block_table, "block_table", torch.int32, dims=2)
+    if tables.numel() == 0 or block_table.shape[0] < n or block_table.shape[1] == 0 or page_size <= 0:
+        raise KernelError(f"tables {tuple(tables.shape)}, block_table {tuple(block_table.shape)} and page_size {page_size} do not fit {n} slots")
+    native.call("b200_slot_load_maps", at, records.shape[0], *given, tables_at, tables.shape[0], tables.shape[1], block_at,
+                block_table.shape[1], n, int(page_size), native.stream_ptr())

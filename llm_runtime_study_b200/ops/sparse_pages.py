@@ -9,20 +9,24 @@ the batch or on where a prompt was cut.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import native
 from ..errors import KernelError
-from .native import c_float, c_int, c_void_p, ptr, require, require_here, stream_ptr, tag
+from .native import c_float, c_int, c_void_p, pointer, stream_ptr
 
 _TABLE = {
     "b200_sparse_pages_head_dim": [],
     "b200_page_bounds": [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 6 + [c_void_p],
-    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 12 + [c_void_p],
+    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p, c_void_p] + [c_int] * 11 + [c_void_p],
+    "b200_choose_pages_tiles": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 11 + [c_void_p],
     "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p],
 }
 SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
 DTYPES = (torch.float32, torch.bfloat16)
+SCORE_CTAS = 8              # CTAs a multiprocessor gets of the scores of single tokens, one after the other
 MAX_TABLE_WIDTH = 51200      # pages of a row whose scores fit into a CTA's shared memory
 
 
@@ -30,6 +34,7 @@ def supported(head_dim: int) -> bool:
     return head_dim % 16 == 0 and 16 <= head_dim <= 256
 
 
+@lru_cache(maxsize=None)
 def library_name(head_dim: int) -> str:
     if not supported(head_dim):
         raise KernelError(f"head size {head_dim} is not a multiple of 16 up to 256")
@@ -48,33 +53,37 @@ def build(head_dim: int) -> None:
     build_library(name, SOURCES, native.library_defines(name))
 
 
-def _pool(t: torch.Tensor, name: str, dims: int, dtype=None) -> tuple[int, ...]:
-    require(t, name, dtype=dtype or DTYPES, dims=dims)
-    require_here(t, name, 16)
-    if t.numel() == 0:
-        raise KernelError(f"{name} of shape {tuple(t.shape)} holds nothing")
-    return tuple(t.shape)
+def _pool(t: torch.Tensor, name: str) -> int:
+    """The address of pages of keys, which set the type of everything beside them."""
+
+    if not isinstance(t, torch.Tensor) or t.dtype not in native.DTYPE_TAG:
+        native.require(t, name, dtype=DTYPES)
+    return pointer(t, name, t.dtype, dims=4, align=16)
 
 
-def _rows(positions, token_entry, block_table, n: int) -> None:
-    require(positions, "positions", dtype=torch.int32, shape=(n,))
-    require(token_entry, "token_entry", dtype=torch.int32, shape=(n,))
-    require(block_table, "block_table", dtype=torch.int32, dims=2)
-    if block_table.numel() == 0:
+def _sizes(*sizes: int) -> None:
+    if min(sizes) <= 0:
+        raise KernelError(f"pages of sizes {sizes} hold nothing")
+
+
+def _rows(positions, token_entry, block_table, n: int) -> tuple[int, int, int, int]:
+    """Addresses of the rows' positions and entries and of the block table, and the table's width."""
+
+    given = (pointer(positions, "positions", torch.int32, shape=(n,)), pointer(token_entry, "token_entry", torch.int32, shape=(n,)),
+             pointer(block_table, "block_table", torch.int32, dims=2), block_table.shape[1])
+    if not block_table.numel():
         raise KernelError(f"a block table of shape {tuple(block_table.shape)} has no cells")
-    for t, name in ((positions, "positions"), (token_entry, "token_entry"), (block_table, "block_table")):
-        require_here(t, name)
+    return given
 
 
-def _query(q: torch.Tensor, kv_heads: int, head_dim: int, dtype) -> tuple[int, int]:
-    require(q, "q", dtype=dtype, dims=3)
-    require_here(q, "q", 16)
+def _query(q: torch.Tensor, kv_heads: int, head_dim: int, dtype) -> tuple[int, int, int]:
+    at = pointer(q, "q", dtype, dims=3, align=16)
     n, heads, d = q.shape
     if d != head_dim or heads == 0 or heads % kv_heads:
         raise KernelError(f"q {tuple(q.shape)} does not fit {kv_heads} key heads of {head_dim}")
     if n * heads >= 1 << 31:
         raise KernelError(f"{n} rows of {heads} heads are too many for one launch")
-    return n, heads
+    return at, n, heads
 
 
 def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
@@ -84,42 +93,40 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
     ``[pages, kv heads, 2, d]`` (low, high) of the same type; ``max_q_len``: the most new tokens of an entry (a hint for the
     launch).  Pages that are not full keep what they have; a NaN among a channel's keys makes both bounds NaN."""
 
-    pages, kv_heads, page_size, d = _pool(keys, "keys", 4)
+    at = _pool(keys, "keys")
+    pages, kv_heads, page_size, d = keys.shape
     library = library_name(d)
-    require(bounds, "bounds", dtype=keys.dtype, shape=(pages, kv_heads, 2, d))
-    require_here(bounds, "bounds", 16)
-    require(kv_len, "kv_len", dtype=torch.int32, dims=1)
+    _sizes(pages, kv_heads, page_size)
+    bounds_at = pointer(bounds, "bounds", keys.dtype, shape=(pages, kv_heads, 2, d), align=16)
+    kv_len_at = pointer(kv_len, "kv_len", torch.int32, dims=1)
     entries = kv_len.shape[0]
-    require(block_table, "block_table", dtype=torch.int32, dims=2)
-    require(q_start, "q_start", dtype=torch.int32, shape=(entries + 1,))
-    for t, name in ((block_table, "block_table"), (q_start, "q_start"), (kv_len, "kv_len")):
-        require_here(t, name)
-    if block_table.shape[0] != entries or block_table.numel() == 0 and entries:
+    q_start_at = pointer(q_start, "q_start", torch.int32, shape=(entries + 1,))
+    table_at = pointer(block_table, "block_table", torch.int32, dims=2)
+    rows, width = block_table.shape
+    if rows != entries or (entries and not width):
         raise KernelError(f"a block table of shape {tuple(block_table.shape)} does not fit {entries} entries")
     if max_q_len < 0:
         raise KernelError("max_q_len must not be negative")
-    if not entries or not max_q_len:
-        return
-    native.call("b200_page_bounds", ptr(keys), ptr(bounds), ptr(block_table), block_table.shape[1], ptr(q_start), ptr(kv_len), entries,
-                -(-max_q_len // page_size), kv_heads, page_size, pages, tag(keys.dtype), stream_ptr(), library=library)
+    if entries and max_q_len:
+        native.call("b200_page_bounds", at, bounds_at, table_at, width, q_start_at, kv_len_at, entries, -(-max_q_len // page_size), kv_heads,
+                    page_size, pages, native.DTYPE_TAG[keys.dtype], stream_ptr(), library=library)
 
 
+@lru_cache(maxsize=4096)
 def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[int, int]:
-    """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each; a cluster shares out
-    the pages of few rows, and the shared memory that the scores of many pages need."""
+    """(tiles of eight rows or not, CTAs that share out a row's or a tile's pages).  Tiles where entries have several rows each, in
+    clusters where few of them would not fill the GPU or the scores of many pages not fit; for single tokens CTAs of 64 pages at
+    least, some for every multiprocessor."""
 
-    def fill(units: int, cluster: int) -> int:
-        while cluster < 8 and 2 * cluster * units <= 2 * native.sm_count() and width // (2 * cluster) >= 64:
-            cluster *= 2
-        return cluster
-
+    sms = native.sm_count()
     if rows >= 2 * entries:
-        sums, cluster = 2 * head_dim * 64, 1
-        while cluster < 8 and sums + 32 * width // cluster > 100 * 1024:
+        units, sums, cluster = -(-rows // 8) * kv_heads, 2 * head_dim * 64, 1
+        while cluster < 8 and (sums + 32 * width // cluster > 100 * 1024
+                               or (2 * cluster * units <= 2 * sms and width // (2 * cluster) >= 64)):
             cluster *= 2
         if sums + 32 * width // cluster <= 200 * 1024:
-            return 1, fill(-(-rows // 8) * kv_heads, cluster)
-    return 0, fill(rows * kv_heads, 1)
+            return True, cluster
+    return False, max(1, min(-(-width // 64), SCORE_CTAS * sms // (rows * kv_heads)))
 
 
 def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor,
@@ -132,27 +139,37 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
     taken, a NaN (an infinite bound that meets a sum of 0 gives one) ranks first.  A page that is not held (an id that is none) is
     not chosen."""
 
-    pages, kv_heads, two, d = _pool(bounds, "bounds", 4)
+    at = _pool(bounds, "bounds")
+    pages, kv_heads, two, d = bounds.shape
     library = library_name(d)
+    _sizes(pages, kv_heads)
     if two != 2:
         raise KernelError(f"bounds of shape {tuple(bounds.shape)} are not [pages, kv heads, 2, d]")
-    n, heads = _query(q, kv_heads, d, bounds.dtype)
-    _rows(positions, token_entry, block_table, n)
+    q_at, n, heads = _query(q, kv_heads, d, bounds.dtype)
+    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n)
     if page_size <= 0 or first < 0 or last < 1 or budget < first + last:
         raise KernelError(f"page_size {page_size}, budget {budget}, first {first} and last {last}: the budget holds the first pages and "
                           "the last ones, of which there is one at least")
-    if block_table.shape[1] > MAX_TABLE_WIDTH:
-        raise KernelError(f"block tables of more than {MAX_TABLE_WIDTH} pages are not taken: {block_table.shape[1]}")
+    if width > MAX_TABLE_WIDTH:
+        raise KernelError(f"block tables of more than {MAX_TABLE_WIDTH} pages are not taken: {width}")
     if n * kv_heads * budget >= 1 << 40:
         raise KernelError(f"a budget of {budget} pages for {n} rows of {kv_heads} heads is too much")
     chosen = torch.empty((n, kv_heads, budget), dtype=torch.int32, device=q.device)
     if n:
-        native.call("b200_choose_pages", ptr(q), ptr(bounds), ptr(positions), ptr(token_entry), ptr(block_table), block_table.shape[1],
-                    ptr(chosen), n, block_table.shape[0], heads, kv_heads, int(page_size), pages, int(budget), int(first), int(last),
-                    *choose_shape(n, block_table.shape[0], kv_heads, block_table.shape[1], d), tag(q.dtype), stream_ptr(), library=library)
+        entries = block_table.shape[0]
+        tiles, shares = choose_shape(n, entries, kv_heads, width, d)
+        given = (q_at, at, positions_at, entry_at, table_at, width, chosen.data_ptr())
+        sizes = (n, entries, heads, kv_heads, int(page_size), pages, int(budget), int(first), int(last), shares,
+                 native.DTYPE_TAG[bounds.dtype], stream_ptr())
+        if tiles:
+            native.call("b200_choose_pages_tiles", *given, *sizes, library=library)
+        else:
+            keys = torch.empty(n * kv_heads * width, dtype=torch.int32, device=q.device)
+            native.call("b200_choose_pages", *given, keys.data_ptr(), *sizes, library=library, launches=2)
     return chosen
 
 
+@lru_cache(maxsize=4096)
 def attention_parts(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> int:
     """Into how many CTAs of a cluster the list of a row and kv head is cut: 1, 2, 4 or 8.  float32: from the list's length alone, so
     that the order of the sums does not depend on the batch.  bfloat16: until the GPU is full, no part shorter than 128 keys."""
@@ -175,22 +192,23 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     ``values`` are ``[pages, kv heads, page size, d]``.  Keys behind the position and pages that are not held are neither read nor
     counted; a row without a key (or without a score above minus infinity) gives zeros."""
 
-    pages, kv_heads, page_size, d = _pool(keys, "keys", 4)
+    at = _pool(keys, "keys")
+    pages, kv_heads, page_size, d = shape = keys.shape
     library = library_name(d)
-    require(values, "values", dtype=keys.dtype, shape=keys.shape)
-    require_here(values, "values", 16)
-    n, heads = _query(q, kv_heads, d, keys.dtype)
-    _rows(positions, token_entry, block_table, n)
-    require(chosen, "chosen", dtype=torch.int32, dims=3)
-    require_here(chosen, "chosen")
-    if tuple(chosen.shape[:2]) != (n, kv_heads) or chosen.shape[2] == 0:
+    _sizes(pages, kv_heads, page_size)
+    values_at = pointer(values, "values", keys.dtype, shape=shape, align=16)
+    q_at, n, heads = _query(q, kv_heads, d, keys.dtype)
+    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n)
+    chosen_at = pointer(chosen, "chosen", torch.int32, dims=3)
+    rows, of_heads, budget = chosen.shape
+    if rows != n or of_heads != kv_heads or not budget:
         raise KernelError(f"chosen of shape {tuple(chosen.shape)} does not fit {n} rows of {kv_heads} key heads")
-    if chosen.shape[2] * page_size > 1 << 30:
-        raise KernelError(f"{chosen.shape[2]} pages of {page_size} tokens a row are too many")
+    if budget * page_size > 1 << 30:
+        raise KernelError(f"{budget} pages of {page_size} tokens a row are too many")
     out = torch.empty_like(q)
     if n:
-        native.call("b200_attend_chosen", ptr(q), ptr(keys), ptr(values), ptr(chosen), ptr(positions), ptr(token_entry), ptr(block_table),
-                    block_table.shape[1], ptr(out), n, block_table.shape[0], heads, kv_heads, page_size, pages, chosen.shape[2],
-                    float(scale), attention_parts(n, heads, kv_heads, chosen.shape[2], page_size, q.dtype), tag(q.dtype), stream_ptr(),
+        native.call("b200_attend_chosen", q_at, at, values_at, chosen_at, positions_at, entry_at, table_at, width, out.data_ptr(), n,
+                    block_table.shape[0], heads, kv_heads, page_size, pages, budget, float(scale),
+                    attention_parts(n, heads, kv_heads, budget, page_size, keys.dtype), native.DTYPE_TAG[keys.dtype], stream_ptr(),
                     library=library)
     return out

@@ -11,11 +11,17 @@ from ..ops import attention_bf16
 from ..ops import attention_rules
 from ..ops import functional as F
 from ..ops import mixer_steps as M
+from ..ops import sparse_pages
 from ..weights.checkpoint import TensorSpec
 from ..weights.view import TensorView
 from .base import MIXERS, NORMS, POSITION_ENCODINGS, Mixer, PagedKV, PagedTensors, Runtime
 from .linear import Projection
 from .norm import RMSNorm
+
+
+# Of the pages that a query may read (``Runtime.attention_pages``), these are always among them: the sequence's first one, which
+# attention falls back to, and the last two (the page being filled, whose bounds are not known yet, and the one before).
+FIRST_PAGES, LAST_PAGES = 1, 2
 
 
 @MIXERS.register("gqa_attention")
@@ -28,6 +34,10 @@ class GroupedQueryAttention(Mixer):
     291-302; scale ``1/sqrt(head_dim)`` unless given, :95-99).
 
     Every size is a parameter; the part does not know the model around it.
+
+    With ``attention_pages`` in the runtime, and no window, every query reads at most so many pages of the sequence: those whose
+    keys can have the highest scores by the bounds kept for each page (``ops/sparse_pages.py``).  Which ones depends on the query
+    and its position alone, so prompts may be cut, batched and computed anew as before.
     """
 
     def __init__(
@@ -48,6 +58,7 @@ class GroupedQueryAttention(Mixer):
         # A layer that reads keys and values written by an earlier layer: it has a
         # query and an output projection only, and writes nothing into the cache.
         self.shares_kv = bool(shares_kv)
+        self.attention_pages: int | None = None      # known once the part is loaded
         self.q_norm = NORMS.build(qk_norm) if qk_norm else None
         self.k_norm = NORMS.build(qk_norm) if qk_norm else None
         if qk_norm and not isinstance(self.q_norm, RMSNorm):
@@ -84,6 +95,7 @@ class GroupedQueryAttention(Mixer):
 
     def load(self, tensors: Mapping[str, torch.Tensor], runtime: Runtime) -> None:
         self.runtime = runtime
+        self.attention_pages = None if self.window else runtime.attention_pages
         names = ("q_proj",) if self.shares_kv else ("q_proj", "k_proj", "v_proj")
         self.qkv_proj = Projection(
             [tensors[f"{n}.weight"] for n in names],
@@ -101,7 +113,10 @@ class GroupedQueryAttention(Mixer):
 
     # --------------------------------------------------------------- cache
     def cache_requirement(self) -> PagedKV | None:
-        return None if self.shares_kv else PagedKV(self.num_kv_heads, self.head_dim, self.window)
+        if self.shares_kv:
+            return None
+        bounds = (("bounds", (self.num_kv_heads, 2, self.head_dim)),) if self.attention_pages is not None else ()
+        return PagedKV(self.num_kv_heads, self.head_dim, self.window, page_tensors=bounds)
 
     # ------------------------------------------------------------- forward
     adds_to_residual = True
@@ -112,7 +127,8 @@ class GroupedQueryAttention(Mixer):
         rotary = self.position.rotary_parameters() if self.position is not None else None
         table = ctx.block_table(cache.group)
         written_kv_heads = 0 if self.shares_kv else self.num_kv_heads
-        if (ctx.all_decode and qkv.dtype == torch.bfloat16 and qkv.shape[0] == ctx.num_entries and not self.shares_kv
+        bounds = cache.tensors.get("bounds") if self.attention_pages is not None else None
+        if (bounds is None and ctx.all_decode and qkv.dtype == torch.bfloat16 and qkv.shape[0] == ctx.num_entries and not self.shares_kv
                 and (self.position is None or rotary is not None)
                 and attention_bf16.fused_decode_supported(self.head_dim, cache.page_size, self.window or 0, rotary[1] if rotary else 0)):
             # one new token per request: the decode kernel normalises, rotates and stores q, k and v itself
@@ -142,8 +158,21 @@ class GroupedQueryAttention(Mixer):
             block_table=None if self.shares_kv else table, page_size=cache.page_size,
             k_pool=None if self.shares_kv else cache.keys, v_pool=None if self.shares_kv else cache.values,
         )
-        out = ctx.attention(q, cache, scale=self.scale, window=self.window or 0)
+        if bounds is None:
+            out = ctx.attention(q, cache, scale=self.scale, window=self.window or 0)
+        else:
+            out = self._attend_chosen(q, ctx, cache, table, bounds)
         return self.o_proj(out.view(out.shape[0], -1), torch.float32, add_to=residual, next_norm=next_norm)
+
+    def _attend_chosen(self, q: torch.Tensor, ctx: Any, cache: Any, table: torch.Tensor, bounds: torch.Tensor) -> torch.Tensor:
+        if not self.shares_kv:
+            sparse_pages.page_bounds(cache.keys, bounds, block_table=table, q_start=ctx.q_start, kv_len=ctx.kv_len, max_q_len=ctx.max_q_len)
+        if q.dtype == torch.bfloat16 and not ctx.all_decode and ctx.max_kv_len <= self.attention_pages * cache.page_size:
+            return ctx.attention(q, cache, scale=self.scale)      # portions of prompts that no row would choose from
+        rows = {"positions": ctx.positions, "token_entry": ctx.token_entry, "block_table": table}
+        chosen = sparse_pages.choose_pages(q, bounds, page_size=cache.page_size, budget=self.attention_pages, first=FIRST_PAGES,
+                                           last=LAST_PAGES, **rows)
+        return sparse_pages.paged_attention_chosen(q, cache.keys, cache.values, chosen, scale=self.scale, **rows)
 
 
 @MIXERS.register("sink_attention")

@@ -46,10 +46,13 @@ from ..weights.checkpoint import TensorSpec
 class Runtime:
     """Where and in which type a model runs.  ``dtype`` is the storage type of
     matrices, activations and the cache: ``torch.bfloat16`` (serving) or
-    ``torch.float32`` (verification; FFMA only, no reduced-precision matrix mode)."""
+    ``torch.float32`` (verification; FFMA only, no reduced-precision matrix mode).  ``attention_pages``: the most
+    pages of keys and values that a query of a layer over the whole sequence reads (``None``: all of them); kinds
+    that can choose pages keep to it, others ignore it."""
 
     device: torch.device
     dtype: torch.dtype
+    attention_pages: int | None = None
 
     def place_matrix(self, t: torch.Tensor) -> torch.Tensor:
         """To the device as stored (for a mapped file: straight from its pages), then to the run type there."""
@@ -70,12 +73,14 @@ class PagedTensors:
     is held as ``[pages, a, page_size, b, ...]`` (one (page, a) tile is contiguous), one of shape ``(a,)`` as
     ``[pages, page_size, a]``.  ``window`` (tokens) bounds how far back the mixer reads; pages wholly behind
     it are given back early and the group's pool is sized for the window rather than for whole sequences.
-    ``page_size`` is the group's own (``None``: the cache manager's default).  Layers with equal
-    requirements share a group of pages: one page id addresses the same positions in each of them."""
+    ``page_size`` is the group's own (``None``: the cache manager's default).  ``page_tensors`` are kept once per page
+    instead: ``[pages, *shape]``.  Layers with equal requirements share a group of pages: one page id addresses the same
+    positions in each of them."""
 
     tensors: tuple[tuple[str, tuple[int, ...]], ...]
     window: int | None = None
     page_size: int | None = None
+    page_tensors: tuple[tuple[str, tuple[int, ...]], ...] = ()
 
 
 @dataclass(frozen=True)
@@ -85,10 +90,12 @@ class PagedKV(PagedTensors):
     num_kv_heads: int = 0
     head_dim: int = 0
 
-    def __init__(self, num_kv_heads: int, head_dim: int, window: int | None = None, page_size: int | None = None) -> None:
+    def __init__(self, num_kv_heads: int, head_dim: int, window: int | None = None, page_size: int | None = None,
+                 page_tensors: tuple[tuple[str, tuple[int, ...]], ...] = ()) -> None:
         object.__setattr__(self, "tensors", (("keys", (num_kv_heads, head_dim)), ("values", (num_kv_heads, head_dim))))
         object.__setattr__(self, "window", window)
         object.__setattr__(self, "page_size", page_size)
+        object.__setattr__(self, "page_tensors", tuple(page_tensors))
         object.__setattr__(self, "num_kv_heads", num_kv_heads)
         object.__setattr__(self, "head_dim", head_dim)
 

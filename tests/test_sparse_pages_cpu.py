@@ -14,28 +14,23 @@ from tests.plain import sparse_pages_plain as plain
 def host(monkeypatch):
     """The operators with CPU tensors taken for CUDA ones; a launch is an error of the test."""
 
-    def require(t, name, *, dtype=None, shape=None, dims=None):
-        if not t.is_contiguous():
-            raise KernelError(f"{name} must be contiguous")
-        if dtype is not None and t.dtype not in (dtype if isinstance(dtype, (tuple, list)) else (dtype,)):
-            raise KernelError(f"{name} has dtype {t.dtype}")
-        if dims is not None and t.dim() != dims:
-            raise KernelError(f"{name} has {t.dim()} dimensions")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise KernelError(f"{name} has shape {tuple(t.shape)}")
-        return t
-
-    def here(t, name, align=4):
+    def pointer(t, name, dtype, *, shape=None, dims=None, align=4):
+        if t.dtype is not dtype or not t.is_contiguous() or (shape is not None and t.shape != shape) or (dims is not None and t.dim() != dims):
+            raise KernelError(name)
         if t.data_ptr() % align:
             raise KernelError(f"{name} must start on a multiple of {align} bytes")
+        return t.data_ptr()
+
+    def require(t, name, *, dtype=None, **_):
+        if t.dtype not in (dtype if isinstance(dtype, (tuple, list)) else (dtype,)):
+            raise KernelError(f"{name} has dtype {t.dtype}")
 
     launched = []
     for module in (page_tables, sparse_pages):
-        monkeypatch.setattr(module, "require", require)
-        monkeypatch.setattr(module, "stream_ptr" if module is sparse_pages else "ptr", lambda *a: 0)
-    monkeypatch.setattr(sparse_pages, "require_here", here)
-    monkeypatch.setattr(native, "require_here", here)
-    monkeypatch.setattr(native, "stream_ptr", lambda: 0)
+        monkeypatch.setattr(module, "pointer", pointer)
+    monkeypatch.setattr(native, "require", require)
+    for module in (native, sparse_pages):
+        monkeypatch.setattr(module, "stream_ptr", lambda: 0)
     monkeypatch.setattr(native, "call", lambda *a, **k: launched.append(a[0]))
     return launched
 
@@ -169,19 +164,26 @@ def test_cpu_tensors_are_refused():
 
 
 def test_tensors_of_another_device_are_refused(monkeypatch):
-    class Elsewhere:
-        is_cuda, device = True, torch.device("cuda", 1)
+    class Elsewhere(torch.Tensor):
+        is_cuda, index = True, 1
+        device = torch.device("cuda", 1)
 
-        def data_ptr(self):
-            return 64
+        def get_device(self):
+            return self.index
 
+    t = torch.zeros(64, dtype=torch.int32).as_subclass(Elsewhere)
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     with pytest.raises(KernelError, match="current device"):
-        native.require_here(Elsewhere(), "q")
-    Elsewhere.device = torch.device("cuda", 0)
-    native.require_here(Elsewhere(), "q", 16)
+        native.pointer(t, "q", torch.int32)
+    Elsewhere.index = 0
+    assert native.pointer(t, "q", torch.int32, shape=(64,), dims=1) == t.data_ptr()
+    for wrong in (dict(shape=(63,)), dict(dims=2)):
+        with pytest.raises(KernelError):
+            native.pointer(t, "q", torch.int32, **wrong)
+    with pytest.raises(KernelError, match="dtype"):
+        native.pointer(t, "q", torch.int64)
     with pytest.raises(KernelError, match="multiple"):
-        native.require_here(Elsewhere(), "q", 128)
+        native.pointer(t[1:], "q", torch.int32, align=16)
 
 
 def test_a_page_s_score_bounds_the_scores_of_its_keys():

@@ -169,6 +169,17 @@ def test_chosen_pages(dtype, case):
     assert torch.equal(got.cpu(), cache.plain_choose(budget, first, last))
 
 
+@pytest.mark.parametrize("rows", [1, 11])
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_chosen_pages_at_every_head_size(dtype, d, rows):
+    """Single tokens of several requests, and rows of one."""
+
+    lengths, counts = ([150, 77, 9], [1, 1, 1]) if rows == 1 else ([150], [rows])
+    cache = Cache(lengths, counts, heads=6, kv_heads=2, d=d, page=4, dtype=dtype, seed=d)
+    assert torch.equal(cache.choose(7, 1, 2).cpu(), cache.plain_choose(7, 1, 2))
+
+
 @pytest.mark.parametrize("rows", [1, 3])
 def test_many_pages(rows):
     """More pages than a CTA has threads many times over, against a vectorised form."""
