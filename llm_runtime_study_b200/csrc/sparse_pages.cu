@@ -93,7 +93,6 @@ struct ChooseArgs {
   const int* token_entry;
   const int* block_table;
   int* chosen;
-  uint32_t* keys;          // scratch of the scores of single tokens, [rows][kv_heads][table_width]
   int table_width, rows, entries, q_heads, kv_heads, page_size, num_pages, budget, first, last, cluster;
 };
 
@@ -251,115 +250,120 @@ template <typename T> struct ScoreLanes {
   static constexpr int at_once = 32 / lanes * ahead;                            // pages of a warp
 };
 
-// Single tokens, scores: a.cluster CTAs per (row, kv head) share out its pages, warp by warp; a team of lanes holds U and D in
-// registers and reads a page's bounds 16 bytes a lane, the next pages' ones before these are summed.  Scores are summed in 64 bits
-// and rounded once: the products of bfloat16 numbers are exact there, so neither the order of the sum nor its spread over lanes moves
-// a page across the border.  What bounds it is the reading of the bounds.
+__device__ __forceinline__ void store_in_cluster(uint32_t address, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(address), "r"(v) : "memory");
+}
+
+// Single tokens: a cluster per (row, kv head), whose warps share out the pages; a team of lanes holds U and D in registers and reads
+// a page's bounds 16 bytes a lane, the next pages' ones before these are summed.  Every score's key goes into the first CTA's shared
+// memory, which then chooses.  Scores are summed in 64 bits and rounded once: the products of bfloat16 numbers are exact there, so
+// neither the order of the sum nor its spread over lanes moves a page across the border.
 template <typename T> __global__ void __launch_bounds__(kChooseThreads, ScoreLanes<T>::values <= 8 ? 2 : 1)
-score_pages_kernel(const __grid_constant__ ChooseArgs a) {
+choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
   using L = Vec<T>;
   using R = ScoreLanes<T>;
   constexpr int A = R::ahead;
-  pdl_launch_dependents();       // the choice comes next, and does nothing before its wait
+  extern __shared__ uint32_t keys[];
+  __shared__ uint32_t scratch[select_words(kChooseWarps)];
+  if (a.cluster > 1) cluster_arrive();
+  pdl_trigger();
   pdl_wait();
   const int share = blockIdx.x % a.cluster, unit = blockIdx.x / a.cluster, lane = threadIdx.x & 31;
   const int row = unit / a.kv_heads, head = unit % a.kv_heads;
   const int entry = a.token_entry[row], seen = visible_pages(a, a.positions[row], entry);
   const int from = (share * kChooseWarps + (threadIdx.x >> 5)) * R::at_once, stride = a.cluster * kChooseWarps * R::at_once;
-  if (seen <= a.budget || from >= seen) return;      // nothing to choose from, or nothing left of it
-  const int* table = a.block_table + static_cast<size_t>(entry) * a.table_width;
-  const int team = lane / R::lanes, part = lane % R::lanes;
-  // page j of the team in a round is from + team * A + j; ids are asked for a round before the bounds that they lead to
-  int ids[A];
-#pragma unroll
-  for (int j = 0; j < A; ++j) ids[j] = from + team * A + j < seen ? table[from + team * A + j] : -1;
-  typename L::type low[A][R::per_lane], high[A][R::per_lane];
-  bool is[A];
-  auto fetch = [&]() {
-#pragma unroll
-    for (int j = 0; j < A; ++j) {
-      is[j] = is_held(a, ids[j]);
-      const typename L::type* at = reinterpret_cast<const typename L::type*>(
-          static_cast<const T*>(a.bounds) + (static_cast<size_t>(is[j] ? ids[j] : 0) * a.kv_heads + head) * 2 * kDim);
-#pragma unroll
-      for (int i = 0; i < R::per_lane; ++i) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
-    }
+  const int* table = a.block_table + static_cast<size_t>(seen > 0 ? entry : 0) * a.table_width;
+  const uint32_t keys_at = a.cluster > 1 ? in_cluster(shared_address(keys), 0) : 0;
+  auto put = [&](int p, uint32_t key) {
+    if (a.cluster > 1) store_in_cluster(keys_at + p * 4, key); else keys[p] = key;
   };
-  double u[R::values], d[R::values];
-  const int group = a.q_heads / a.kv_heads;
-  const typename L::type* q = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim);
+  if (a.cluster > 1) cluster_wait();          // every CTA of the cluster has started
+  if (seen <= a.budget) {                     // nothing to choose from: which pages are held is enough
+    for (int p = share * kChooseThreads + threadIdx.x; p < seen; p += a.cluster * kChooseThreads) put(p, is_held(a, table[p]) ? kKeyAlways : kKeyNone);
+  } else {
+    const int team = lane / R::lanes, part = lane % R::lanes;
+    // page j of the team in a round is from + team * A + j; ids are asked for a round before the bounds that they lead to
+    int ids[A];
 #pragma unroll
-  for (int i = 0; i < R::values; ++i) u[i] = d[i] = 0;
-  for (int h = 0; h < group; ++h) {
+    for (int j = 0; j < A; ++j) ids[j] = from + team * A + j < seen ? table[from + team * A + j] : -1;
+    typename L::type low[A][R::per_lane], high[A][R::per_lane];
+    bool is[A];
+    auto fetch = [&]() {
 #pragma unroll
-    for (int i = 0; i < R::per_lane; ++i) {
-      float v[L::n];
-      L::unpack(q[h * R::chunks + part + i * R::lanes], v);
+      for (int j = 0; j < A; ++j) {
+        is[j] = is_held(a, ids[j]);
+        const typename L::type* at = reinterpret_cast<const typename L::type*>(
+            static_cast<const T*>(a.bounds) + (static_cast<size_t>(is[j] ? ids[j] : 0) * a.kv_heads + head) * 2 * kDim);
 #pragma unroll
-      for (int x = 0; x < L::n; ++x) add_part(v[x], u[i * L::n + x], d[i * L::n + x]);
-    }
-  }
-  uint32_t* keys = a.keys + static_cast<size_t>(unit) * a.table_width;
-  fetch();
-  // the trip count is the same for all lanes: they exchange sums
-  for (int base = from; base < seen; base += stride) {
-    double sum[A];
-    uint32_t held = 0;
+        for (int i = 0; i < R::per_lane; ++i) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
+      }
+    };
+    double u[R::values], d[R::values];
+    const int group = a.q_heads / a.kv_heads;
+    const typename L::type* q = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim);
 #pragma unroll
-    for (int j = 0; j < A; ++j) {
-      if (is[j]) held |= 1u << j;
-      double other = 0;
-      sum[j] = 0;
+    for (int i = 0; i < R::values; ++i) u[i] = d[i] = 0;
+    for (int h = 0; h < group; ++h) {
 #pragma unroll
       for (int i = 0; i < R::per_lane; ++i) {
-        float lo[L::n], hi[L::n];
-        L::unpack(low[j][i], lo);
-        L::unpack(high[j][i], hi);
+        float v[L::n];
+        L::unpack(q[h * R::chunks + part + i * R::lanes], v);
 #pragma unroll
-        for (int x = 0; x < L::n; ++x) {
-          sum[j] = fma(static_cast<double>(hi[x]), u[i * L::n + x], sum[j]);
-          other = fma(static_cast<double>(lo[x]), d[i * L::n + x], other);
-        }
+        for (int x = 0; x < L::n; ++x) add_part(v[x], u[i * L::n + x], d[i * L::n + x]);
       }
-      sum[j] += other;
     }
-    const int next = base + stride + team * A;
-#pragma unroll
-    for (int j = 0; j < A; ++j) ids[j] = next + j < seen ? table[next + j] : -1;
-    // halves of the team add up halves of its pages, until every lane is left with one page (its place among the team's A: `mine`)
-    int mine = 0, width = R::lanes / 2;
-#pragma unroll
-    for (int n = A; n > 1; n /= 2, width /= 2) {
-      const bool upper = part & width;
-#pragma unroll
-      for (int j = 0; j < n / 2; ++j) {
-        const double give = upper ? sum[j] : sum[j + n / 2], keep = upper ? sum[j + n / 2] : sum[j];
-        sum[j] = keep + __shfl_xor_sync(0xffffffffu, give, width);
-      }
-      mine += upper ? n / 2 : 0;
-    }
-#pragma unroll
-    for (; width >= 1; width /= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], width);
     fetch();
-    const int p = base + team * A + mine;
-    if (part % (R::lanes / A) == 0 && p < seen) keys[p] = key_of(a, p, seen, held >> mine & 1, sum[0]);
+    // the trip count is the same for all lanes: they exchange sums
+    for (int base = from; base < seen; base += stride) {
+      double sum[A];
+      uint32_t held = 0;
+#pragma unroll
+      for (int j = 0; j < A; ++j) {
+        if (is[j]) held |= 1u << j;
+        double other = 0;
+        sum[j] = 0;
+#pragma unroll
+        for (int i = 0; i < R::per_lane; ++i) {
+          float lo[L::n], hi[L::n];
+          L::unpack(low[j][i], lo);
+          L::unpack(high[j][i], hi);
+#pragma unroll
+          for (int x = 0; x < L::n; ++x) {
+            sum[j] = fma(static_cast<double>(hi[x]), u[i * L::n + x], sum[j]);
+            other = fma(static_cast<double>(lo[x]), d[i * L::n + x], other);
+          }
+        }
+        sum[j] += other;
+      }
+      const int next = base + stride + team * A;
+#pragma unroll
+      for (int j = 0; j < A; ++j) ids[j] = next + j < seen ? table[next + j] : -1;
+      // halves of the team add up halves of its pages, until every lane is left with one page (its place among the team's A: `mine`)
+      int mine = 0, width = R::lanes / 2;
+#pragma unroll
+      for (int n = A; n > 1; n /= 2, width /= 2) {
+        const bool upper = part & width;
+#pragma unroll
+        for (int j = 0; j < n / 2; ++j) {
+          const double give = upper ? sum[j] : sum[j + n / 2], keep = upper ? sum[j + n / 2] : sum[j];
+          sum[j] = keep + __shfl_xor_sync(0xffffffffu, give, width);
+        }
+        mine += upper ? n / 2 : 0;
+      }
+#pragma unroll
+      for (; width >= 1; width /= 2) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], width);
+      fetch();
+      const int p = base + team * A + mine;
+      if (part % (R::lanes / A) == 0 && p < seen) put(p, key_of(a, p, seen, held >> mine & 1, sum[0]));
+    }
   }
-}
-
-// Single tokens, choice: a CTA per (row, kv head).
-constexpr int kSelectWarps = 16;
-__global__ void __launch_bounds__(kSelectWarps * 32) select_pages_kernel(const __grid_constant__ ChooseArgs a) {
-  extern __shared__ uint32_t keys[];
-  __shared__ uint32_t scratch[select_words(kSelectWarps)];
-  pdl_trigger();
-  pdl_wait();
-  const int unit = blockIdx.x, row = unit / a.kv_heads, t = threadIdx.x;
-  const int entry = a.token_entry[row], seen = visible_pages(a, a.positions[row], entry);
-  const int* table = a.block_table + static_cast<size_t>(seen > 0 ? entry : 0) * a.table_width;
-  const uint32_t* made = a.keys + static_cast<size_t>(unit) * a.table_width;
-  for (int p = t; p < seen; p += kSelectWarps * 32) keys[p] = seen > a.budget ? made[p] : (is_held(a, table[p]) ? kKeyAlways : kKeyNone);
   __syncthreads();
-  select_pages<kSelectWarps>(keys, seen, a.budget, a.chosen + static_cast<size_t>(unit) * a.budget, scratch, t);
+  if (a.cluster > 1) {
+    cluster_arrive();
+    cluster_wait();
+    if (share != 0) return;
+  }
+  select_pages<kChooseWarps>(keys, seen, a.budget, a.chosen + static_cast<size_t>(unit) * a.budget, scratch, threadIdx.x);
 }
 
 // Rows of prompts: a cluster per (eight rows, kv head), the scores as a product [8 rows, 2 d] x [2 d, pages] on the 64-bit tensor
@@ -369,9 +373,6 @@ __global__ void __launch_bounds__(kSelectWarps * 32) select_pages_kernel(const _
 // scored entry by entry.
 constexpr int kTileRows = 8;
 
-__device__ __forceinline__ void store_in_cluster(uint32_t address, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(address), "r"(v) : "memory");
-}
 
 __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
   asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};\n" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
@@ -478,16 +479,16 @@ constexpr int kChooseSharedBytes = 200 * 1024;
 
 inline bool fits(const ChooseArgs& a) {
   return a.table_width > 0 && a.entries > 0 && a.kv_heads > 0 && a.q_heads > 0 && a.q_heads % a.kv_heads == 0 && a.page_size > 0 &&
-         a.num_pages > 0 && a.first >= 0 && a.last >= 1 && a.budget >= a.first + a.last;
+         a.num_pages > 0 && a.first >= 0 && a.last >= 1 && a.budget >= a.first + a.last &&
+         (a.cluster == 1 || a.cluster == 2 || a.cluster == 4 || a.cluster == 8);
 }
 
 template <typename T> int launch_choose(const ChooseArgs& a, cudaStream_t stream) {
   static DeviceOnce once;
-  const long long units = static_cast<long long>(a.rows) * a.kv_heads, bytes = static_cast<long long>(a.table_width) * 4;
-  if (bytes > kChooseSharedBytes || units * a.cluster > 0x7fffffffll) return B200_ERR_TOO_LARGE;
-  if (const int status = configure_once(once, select_pages_kernel, kChooseSharedBytes)) return status;
-  launch(score_pages_kernel<T>, dim3(static_cast<unsigned>(units * a.cluster)), dim3(kChooseThreads), 0, stream, a);
-  launch(select_pages_kernel, dim3(static_cast<unsigned>(units)), dim3(kSelectWarps * 32), static_cast<size_t>(bytes), stream, a);
+  const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * a.cluster, bytes = static_cast<long long>(a.table_width) * 4;
+  if (bytes > kChooseSharedBytes || ctas > 0x7fffffffll) return B200_ERR_TOO_LARGE;
+  if (const int status = configure_once(once, choose_pages_kernel<T>, kChooseSharedBytes)) return status;
+  launch_clusters(choose_pages_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(kChooseThreads), static_cast<size_t>(bytes), a.cluster, stream, a);
   return launch_status();
 }
 
@@ -517,15 +518,15 @@ extern "C" int b200_page_bounds(const void* keys, void* bounds, const int* block
   return 0;
 }
 
-// keys: scratch of rows * kv_heads * table_width words, shares: CTAs that share out a row's pages.
+// cluster: CTAs of a cluster that share out a row's pages (1, 2, 4 or 8).
 extern "C" int b200_choose_pages(const void* q, const void* bounds, const int* positions, const int* token_entry,
-                                 const int* block_table, int table_width, int* chosen, uint32_t* keys, int rows, int entries, int q_heads,
-                                 int kv_heads, int page_size, int num_pages, int budget, int first, int last, int shares, int dtype,
+                                 const int* block_table, int table_width, int* chosen, int rows, int entries, int q_heads, int kv_heads,
+                                 int page_size, int num_pages, int budget, int first, int last, int cluster, int dtype,
                                  cudaStream_t stream) {
   if (rows <= 0) return 0;
-  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, keys, table_width, rows, entries, q_heads, kv_heads, page_size,
-               num_pages, budget, first, last, shares};
-  if (!fits(a) || shares < 1) return B200_ERR_BAD_SIZE;
+  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, table_width, rows, entries, q_heads, kv_heads, page_size,
+               num_pages, budget, first, last, cluster};
+  if (!fits(a)) return B200_ERR_BAD_SIZE;
   B200_DISPATCH_DTYPE(dtype, T, return launch_choose<T>(a, stream));
   return 0;
 }
@@ -536,9 +537,9 @@ extern "C" int b200_choose_pages_tiles(const void* q, const void* bounds, const 
                                        int kv_heads, int page_size, int num_pages, int budget, int first, int last, int cluster, int dtype,
                                        cudaStream_t stream) {
   if (rows <= 0) return 0;
-  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, nullptr, table_width, rows, entries, q_heads, kv_heads, page_size,
+  ChooseArgs a{q, bounds, positions, token_entry, block_table, chosen, table_width, rows, entries, q_heads, kv_heads, page_size,
                num_pages, budget, first, last, cluster};
-  if (!fits(a) || (cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8)) return B200_ERR_BAD_SIZE;
+  if (!fits(a)) return B200_ERR_BAD_SIZE;
   B200_DISPATCH_DTYPE(dtype, T, return launch_choose_tiles<T>(a, stream));
   return 0;
 }

@@ -72,20 +72,26 @@ def step_maps(
             (entries + 1, num_tokens, num_tokens))
         out = StepMaps(torch.empty((entries, width or table_width), dtype=torch.int32, device=device), q_start, positions, token_entry,
                        torch.empty(num_tokens, dtype=torch.int64, device=device))
+        pointers = [t.data_ptr() for t in (out.block_table, q_start, positions, token_entry, out.slot_map)]
         if not entries:
             q_start.zero_()
-    elif width is not None and out.block_table.shape[-1] != width:
-        raise KernelError(f"out.block_table has {out.block_table.shape[-1]} columns, not {width}")
-    block_table = pointer(out.block_table, "out.block_table", torch.int32, dims=2)
-    rooms = [(out.q_start, "out.q_start", torch.int32, entries + 1), (out.positions, "out.positions", torch.int32, num_tokens),
-             (out.token_entry, "out.token_entry", torch.int32, num_tokens), (out.slot_map, "out.slot_map", torch.int64, num_tokens)]
-    pointers = [None if t is None else pointer(t, name, dtype, dims=1, align=dtype.itemsize) for t, name, dtype, _ in rooms]
-    for t, name, _, least in [(out.block_table, "out.block_table", None, entries), *rooms]:
-        if t is not None and t.shape[0] < least:
-            raise KernelError(f"{name} has room for {t.shape[0]}, {least} are needed")
+    else:
+        if width is not None and out.block_table.shape[-1] != width:
+            raise KernelError(f"out.block_table has {out.block_table.shape[-1]} columns, not {width}")
+        pointers = []
+        for name, dtype, dims, least in (("block_table", torch.int32, 2, entries), ("q_start", torch.int32, 1, entries + 1),
+                                         ("positions", torch.int32, 1, num_tokens), ("token_entry", torch.int32, 1, num_tokens),
+                                         ("slot_map", torch.int64, 1, num_tokens)):
+            t = getattr(out, name)
+            if t is None and dims == 1:
+                pointers.append(None)
+                continue
+            pointers.append(pointer(t, f"out.{name}", dtype, dims=dims, align=dtype.itemsize))
+            if t.shape[0] < least:
+                raise KernelError(f"out.{name} has room for {t.shape[0]}, {least} are needed")
     if entries:
-        native.call("b200_step_maps", at, table_rows, table_width, slots_at, kv_len_at, counts_at, block_table, out.block_table.shape[1],
-                    *pointers, entries, int(page_size), int(num_tokens), native.stream_ptr())
+        native.call("b200_step_maps", at, table_rows, table_width, slots_at, kv_len_at, counts_at, pointers[0], out.block_table.shape[1],
+                    *pointers[1:], entries, int(page_size), int(num_tokens), native.stream_ptr())
     return out
 
 

@@ -20,13 +20,12 @@ from .native import c_float, c_int, c_void_p, pointer, stream_ptr
 _TABLE = {
     "b200_sparse_pages_head_dim": [],
     "b200_page_bounds": [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 6 + [c_void_p],
-    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p, c_void_p] + [c_int] * 11 + [c_void_p],
+    "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 11 + [c_void_p],
     "b200_choose_pages_tiles": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 11 + [c_void_p],
     "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p],
 }
 SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
 DTYPES = (torch.float32, torch.bfloat16)
-SCORE_CTAS = 8              # CTAs a multiprocessor gets of the scores of single tokens, one after the other
 MAX_TABLE_WIDTH = 51200      # pages of a row whose scores fit into a CTA's shared memory
 
 
@@ -114,19 +113,23 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
 
 @lru_cache(maxsize=4096)
 def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[int, int]:
-    """(tiles of eight rows or not, CTAs that share out a row's or a tile's pages).  Tiles where entries have several rows each, in
-    clusters where few of them would not fill the GPU or the scores of many pages not fit; for single tokens CTAs of 64 pages at
-    least, some for every multiprocessor."""
+    """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each; a cluster shares out
+    the pages of a row or a tile where there are few of them (bfloat16, 40 heads over 8 of 128, pages of 32, 65,521 tokens, clusters of
+    1, 2, 4 and 8: 1 request 35, 22, 15 and 12 us, 8 requests 35, 23, 18 and 23, 32 requests 53, 52, 62 and 84), and the shared memory
+    that the scores of many pages need."""
 
-    sms = native.sm_count()
+    def fill(units: int, cluster: int) -> int:
+        while cluster < 8 and 2 * cluster * units <= 2 * native.sm_count() and width // (2 * cluster) >= 64:
+            cluster *= 2
+        return cluster
+
     if rows >= 2 * entries:
-        units, sums, cluster = -(-rows // 8) * kv_heads, 2 * head_dim * 64, 1
-        while cluster < 8 and (sums + 32 * width // cluster > 100 * 1024
-                               or (2 * cluster * units <= 2 * sms and width // (2 * cluster) >= 64)):
+        sums, cluster = 2 * head_dim * 64, 1
+        while cluster < 8 and sums + 32 * width // cluster > 100 * 1024:
             cluster *= 2
         if sums + 32 * width // cluster <= 200 * 1024:
-            return True, cluster
-    return False, max(1, min(-(-width // 64), SCORE_CTAS * sms // (rows * kv_heads)))
+            return True, fill(-(-rows // 8) * kv_heads, cluster)
+    return False, fill(rows * kv_heads, 1)
 
 
 def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor,
@@ -157,15 +160,10 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
     chosen = torch.empty((n, kv_heads, budget), dtype=torch.int32, device=q.device)
     if n:
         entries = block_table.shape[0]
-        tiles, shares = choose_shape(n, entries, kv_heads, width, d)
-        given = (q_at, at, positions_at, entry_at, table_at, width, chosen.data_ptr())
-        sizes = (n, entries, heads, kv_heads, int(page_size), pages, int(budget), int(first), int(last), shares,
-                 native.DTYPE_TAG[bounds.dtype], stream_ptr())
-        if tiles:
-            native.call("b200_choose_pages_tiles", *given, *sizes, library=library)
-        else:
-            keys = torch.empty(n * kv_heads * width, dtype=torch.int32, device=q.device)
-            native.call("b200_choose_pages", *given, keys.data_ptr(), *sizes, library=library, launches=2)
+        tiles, cluster = choose_shape(n, entries, kv_heads, width, d)
+        native.call("b200_choose_pages_tiles" if tiles else "b200_choose_pages", q_at, at, positions_at, entry_at, table_at, width,
+                    chosen.data_ptr(), n, entries, heads, kv_heads, int(page_size), pages, int(budget), int(first), int(last), cluster,
+                    native.DTYPE_TAG[bounds.dtype], stream_ptr(), library=library)
     return chosen
 
 
