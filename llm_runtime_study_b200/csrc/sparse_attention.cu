@@ -414,20 +414,19 @@ template <typename Kernel> int launch_attend(Kernel kernel, const AttendArgs& a,
   return launch_status();
 }
 
-constexpr int kMmaWarps = 4;
-
-template <int NT> int launch_mma(const AttendArgs& a, cudaStream_t stream) {
-  return a.page_size % 16 == 0 ? launch_attend(attend_mma_kernel<NT, kMmaWarps, true>, a, 8 * NT, kMmaWarps, stream)
-                               : launch_attend(attend_mma_kernel<NT, kMmaWarps, false>, a, 8 * NT, kMmaWarps, stream);
+template <int NT, int WARPS> int launch_mma(const AttendArgs& a, cudaStream_t stream) {
+  return a.page_size % 16 == 0 ? launch_attend(attend_mma_kernel<NT, WARPS, true>, a, 8 * NT, WARPS, stream)
+                               : launch_attend(attend_mma_kernel<NT, WARPS, false>, a, 8 * NT, WARPS, stream);
 }
 
 }  // namespace b200
 
 using namespace b200;
 
+// parts: CTAs of a cluster that share out a list; wide: eight warps to a CTA where there is such a kernel (bfloat16).
 extern "C" int b200_attend_chosen(const void* q, const void* keys, const void* values, const int* chosen, const int* positions,
                                   const int* token_entry, const int* block_table, int table_width, void* out, int rows, int entries,
-                                  int q_heads, int kv_heads, int page_size, int num_pages, int budget, float scale, int parts, int dtype,
+                                  int q_heads, int kv_heads, int page_size, int num_pages, int budget, float scale, int parts, int wide, int dtype,
                                   cudaStream_t stream) {
   if (rows <= 0) return 0;
   if (table_width <= 0 || entries <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || page_size <= 0 || num_pages <= 0 ||
@@ -437,7 +436,8 @@ extern "C" int b200_attend_chosen(const void* q, const void* keys, const void* v
   if (dtype == kF32) return launch_attend(attend_streams_kernel, a, Streams::heads, Streams::threads / 32, stream);
   if (dtype != kBF16) return B200_ERR_BAD_DTYPE;
   if constexpr (kDim <= 128) {
-    if (q_heads / kv_heads > 8) return launch_mma<2>(a, stream);
+    if (q_heads / kv_heads > 8) return launch_mma<2, 4>(a, stream);
+    if (wide) return launch_mma<1, 8>(a, stream);
   }
-  return launch_mma<1>(a, stream);
+  return launch_mma<1, 4>(a, stream);
 }

@@ -119,107 +119,154 @@ template <int WARPS> __device__ __forceinline__ void sync_group() {
 }
 constexpr int select_words(int warps) { return 256 + 4 * warps + 3; }
 
-// The `budget` highest of keys[0 .. count) that are not kKeyNone, lower indices first among equals, written in rising order
-// of their indices; -1 behind them.  WARPS warps take part (t: the thread among them), all of the CTA's or one.
-//
-// The border is found digit by digit of eight bits, from the highest bit in which the candidates differ at all (scores lie close
-// together: their upper bits say nothing), until the keys of a digit are wanted all or none: two rounds as a rule.
-template <int WARPS> __device__ void select_pages(const uint32_t* keys, int count, int budget, int* out, uint32_t* scratch, int t) {
-  constexpr int kThreads = WARPS * 32;
-  uint32_t* histogram = scratch;
-  uint32_t* per_warp = scratch + 256;          // four words of each
-  uint32_t* found = per_warp + 4 * WARPS;      // digit, how many are still wanted among its keys, how many those are
-  const int lane = t & 31, warp = t >> 5;
-  uint32_t always = 0, others = 0, least = 0xffffffffu, most = 0;
-  for (int i = t; i < count; i += kThreads) {
+struct Tally {
+  uint32_t always, others;      // how many keys are kKeyAlways, how many are candidates
+  uint32_t least, most;         // of the candidates
+};
+
+// Whether a key is a candidate's.
+__device__ __forceinline__ bool is_other(uint32_t key) { return key != kKeyNone && key != kKeyAlways; }
+
+template <int WARPS> __device__ Tally tally_keys(const uint32_t* keys, int count, uint32_t* scratch, int t) {
+  uint32_t* per_warp = scratch + 256;
+  Tally y{0, 0, 0xffffffffu, 0};
+#pragma unroll 4
+  for (int i = t; i < count; i += WARPS * 32) {
     const uint32_t key = keys[i];
-    if (key == kKeyAlways) ++always;
-    else if (key != kKeyNone) ++others, least = min(least, key), most = max(most, key);
+    y.always += key == kKeyAlways;
+    if (is_other(key)) ++y.others, y.least = min(y.least, key), y.most = max(y.most, key);
   }
-  always = __reduce_add_sync(0xffffffffu, always);
-  others = __reduce_add_sync(0xffffffffu, others);
-  least = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
+  y.always = __reduce_add_sync(0xffffffffu, y.always);
+  y.others = __reduce_add_sync(0xffffffffu, y.others);
+  y.least = __reduce_min_sync(0xffffffffu, y.least);
+  y.most = __reduce_max_sync(0xffffffffu, y.most);
   if (WARPS > 1) {
-    if (lane == 0) per_warp[4 * warp] = always, per_warp[4 * warp + 1] = others, per_warp[4 * warp + 2] = least, per_warp[4 * warp + 3] = most;
     __syncthreads();
-    always = others = most = 0, least = 0xffffffffu;
+    if ((t & 31) == 0) reinterpret_cast<uint4*>(per_warp)[t >> 5] = make_uint4(y.always, y.others, y.least, y.most);
+    __syncthreads();
+    y = Tally{0, 0, 0xffffffffu, 0};
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      always += per_warp[4 * w], others += per_warp[4 * w + 1];
-      least = min(least, per_warp[4 * w + 2]), most = max(most, per_warp[4 * w + 3]);
+      const uint4 v = reinterpret_cast<const uint4*>(per_warp)[w];
+      y.always += v.x, y.others += v.y, y.least = min(y.least, v.z), y.most = max(y.most, v.w);
     }
   }
-  uint32_t threshold = 0, wanted = 0;          // take keys above the threshold, and the first `wanted` equal to it
-  if (always + others > static_cast<uint32_t>(budget)) {
-    wanted = budget - always;                  // the first and the last pages fit into every budget
-    int high = least == most ? 0 : 32 - __clz(least ^ most);       // bits below this one differ
-    threshold = wanted == 0 ? kKeyNaN : (high == 32 ? 0u : most >> high << high);
-    while (wanted > 0 && high > 0) {
-      const int low = max(high - 8, 0);
-      const uint32_t digits = (1u << (high - low)) - 1u;
-      for (int i = t; i < 256; i += kThreads) histogram[i] = 0;
-      sync_group<WARPS>();
-      for (int i = t; i < count; i += kThreads) {
-        const uint32_t key = keys[i];
-        if (key != kKeyNone && key != kKeyAlways && (high == 32 || key >> high == threshold >> high)) atomicAdd(&histogram[key >> low & digits], 1u);
+  return y;
+}
+
+struct Border {
+  uint32_t threshold, wanted;      // take keys above the threshold, and the first `wanted` equal to it
+};
+
+// The border of the `wanted` highest candidates (fewer than there are).  It is found digit by digit of eight bits, from the highest bit
+// in which the candidates differ at all (scores lie close together: their upper bits say nothing), until the keys of a digit are
+// wanted all or none: two rounds as a rule.  WARPS warps take part (t: the thread among them), all of the CTA's or one.
+template <int WARPS> __device__ Border find_border(const uint32_t* keys, int count, const Tally& tally, uint32_t wanted, uint32_t* scratch, int t) {
+  constexpr int kThreads = WARPS * 32;
+  uint32_t* histogram = scratch;
+  uint32_t* found = scratch + 256 + 4 * WARPS;      // digit, how many are still wanted among its keys, how many those are
+  const int lane = t & 31, warp = t >> 5;
+  int high = tally.least == tally.most ? 0 : 32 - __clz(tally.least ^ tally.most);       // bits below this one differ
+  uint32_t threshold = wanted == 0 ? kKeyNaN : (high == 32 ? 0u : tally.most >> high << high);
+  while (wanted > 0 && high > 0) {
+    const int low = max(high - 8, 0);
+    const uint32_t digits = (1u << (high - low)) - 1u;
+    for (int i = t; i < 256; i += kThreads) histogram[i] = 0;
+    sync_group<WARPS>();
+#pragma unroll 4
+    for (int i = t; i < count; i += kThreads) {
+      const uint32_t key = keys[i];
+      if (is_other(key) && (high == 32 || key >> high == threshold >> high)) atomicAdd(&histogram[key >> low & digits], 1u);
+    }
+    sync_group<WARPS>();
+    if (warp == 0) {       // lane l holds the digits 255 - 8 l down to 248 - 8 l
+      uint32_t mine[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i] = histogram[255 - 8 * lane - i], sum += mine[i];
+      uint32_t upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
       }
-      sync_group<WARPS>();
-      if (warp == 0) {       // lane l holds the digits 255 - 8 l down to 248 - 8 l
-        uint32_t mine[8], sum = 0;
+      uint32_t before = upto - sum;
+      if (before < wanted && wanted <= upto) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mine[i] = histogram[255 - 8 * lane - i], sum += mine[i];
-        uint32_t upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t other = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += other;
+        for (int i = 0; i < 8; ++i) {
+          if (before < wanted && wanted <= before + mine[i]) found[0] = 255 - 8 * lane - i, found[1] = wanted - before, found[2] = mine[i];
+          before += mine[i];
         }
-        uint32_t before = upto - sum;
-        if (before < wanted && wanted <= upto) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (before < wanted && wanted <= before + mine[i]) found[0] = 255 - 8 * lane - i, found[1] = wanted - before, found[2] = mine[i];
-            before += mine[i];
-          }
-        }
-      }
-      sync_group<WARPS>();
-      threshold |= found[0] << low;
-      wanted = found[1];
-      high = low;
-      if (wanted == found[2]) {                // all keys of this digit: whatever is not below them
-        threshold = threshold > 0 ? threshold - 1 : 0;
-        wanted = 0;
       }
     }
+    sync_group<WARPS>();
+    threshold |= found[0] << low;
+    wanted = found[1];
+    high = low;
+    if (wanted == found[2]) {                // all keys of this digit: whatever is not below them
+      threshold = threshold > 0 ? threshold - 1 : 0;
+      wanted = 0;
+    }
   }
-  // each warp keeps a run of indices: count, then write at the place the warps before it leave
+  return Border{threshold, wanted};
+}
+
+// Each warp keeps a run of the indices: what a border may take of the runs before a thread's own.
+struct Runs {
+  uint32_t more, same;          // above the threshold, and equal to it
+};
+
+template <int WARPS> __device__ Runs count_runs(const uint32_t* keys, int count, uint32_t threshold, uint32_t* scratch, int t) {
+  constexpr int kThreads = WARPS * 32;
+  uint32_t* per_warp = scratch + 256;
+  const int lane = t & 31, warp = t >> 5;
   const int run = (count + kThreads - 1) / kThreads * 32;
   const int from = warp * run, to = min(from + run, count);
-  uint32_t more = 0, same = 0;
-  if (WARPS > 1) {
-    for (int i = from + lane; i < to; i += 32) more += keys[i] > threshold, same += keys[i] == threshold;
-    more = __reduce_add_sync(0xffffffffu, more);
-    same = __reduce_add_sync(0xffffffffu, same);
-    __syncthreads();                           // the sums of above have been read
-    if (lane == 0) per_warp[2 * warp] = more, per_warp[2 * warp + 1] = same;
+  Runs y{0, 0};
+  if constexpr (WARPS > 1) {     // a single warp has nobody before it
+#pragma unroll 4
+    for (int i = from + lane; i < to; i += 32) y.more += keys[i] > threshold, y.same += keys[i] == threshold;
+    y.more = __reduce_add_sync(0xffffffffu, y.more);
+    y.same = __reduce_add_sync(0xffffffffu, y.same);
+    __syncthreads();               // what was in per_warp has been read
+    if (lane == 0) reinterpret_cast<uint2*>(per_warp)[warp] = make_uint2(y.more, y.same);
     __syncthreads();
-    more = same = 0;
-    for (int w = 0; w < warp; ++w) more += per_warp[2 * w], same += per_warp[2 * w + 1];
+    y = Runs{0, 0};
+    for (int w = 0; w < warp; ++w) {
+      const uint2 v = reinterpret_cast<const uint2*>(per_warp)[w];
+      y.more += v.x, y.same += v.y;
+    }
   }
+  return y;
+}
+
+// The indices of the keys that a border takes, `kept` of them, in rising order; -1 behind them up to `budget`.
+template <int WARPS> __device__ void write_pages(const uint32_t* keys, int count, const Border& border, Runs runs, int kept, int budget, int* out, int t) {
+  constexpr int kThreads = WARPS * 32;
+  const int lane = t & 31, warp = t >> 5;
+  const int run = (count + kThreads - 1) / kThreads * 32;
+  const int from = warp * run, to = min(from + run, count);
   const uint32_t below = (1u << lane) - 1u;
+#pragma unroll 4
   for (int i = from; i < to; i += 32) {
     const uint32_t key = i + lane < to ? keys[i + lane] : kKeyNone;
-    const bool greater = i + lane < to && key > threshold, tie = i + lane < to && key == threshold;
+    const bool greater = i + lane < to && key > border.threshold, tie = i + lane < to && key == border.threshold;
     const uint32_t greater_lanes = __ballot_sync(0xffffffffu, greater), tie_lanes = __ballot_sync(0xffffffffu, tie);
-    const uint32_t ties_before = same + __popc(tie_lanes & below);
-    if (greater || (tie && ties_before < wanted)) out[more + __popc(greater_lanes & below) + min(ties_before, wanted)] = i + lane;
-    more += __popc(greater_lanes);
-    same += __popc(tie_lanes);
+    const uint32_t ties_before = runs.same + __popc(tie_lanes & below);
+    if (greater || (tie && ties_before < border.wanted)) out[runs.more + __popc(greater_lanes & below) + min(ties_before, border.wanted)] = i + lane;
+    runs.more += __popc(greater_lanes);
+    runs.same += __popc(tie_lanes);
   }
-  const int kept = min(always + others, static_cast<uint32_t>(budget));
   for (int i = kept + t; i < budget; i += kThreads) out[i] = -1;
+}
+
+// The `budget` highest of keys[0 .. count) that are not kKeyNone, lower indices first among equals.
+template <int WARPS> __device__ void select_pages(const uint32_t* keys, int count, int budget, int* out, uint32_t* scratch, int t) {
+  const Tally tally = tally_keys<WARPS>(keys, count, scratch, t);
+  const int some = tally.always + tally.others;
+  Border border{0, 0};
+  // the first and the last pages fit into every budget
+  if (some > budget) border = find_border<WARPS>(keys, count, tally, budget - tally.always, scratch, t);
+  write_pages<WARPS>(keys, count, border, count_runs<WARPS>(keys, count, border.threshold, scratch, t), min(some, budget), budget, out, t);
 }
 
 // U and D (see the top of the file).  A NaN gets into the score by way of D.
@@ -228,6 +275,7 @@ __device__ __forceinline__ void add_part(float q, double& up, double& down) {
 }
 template <typename T> __device__ __forceinline__ void parts_of(const T* q, int group, double& up, double& down) {
   up = down = 0;
+#pragma unroll 4
   for (int h = 0; h < group; ++h) add_part(to_float<T>(q[h * kDim]), up, down);
 }
 
@@ -264,7 +312,7 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
   using R = ScoreLanes<T>;
   constexpr int A = R::ahead;
   extern __shared__ uint32_t keys[];
-  __shared__ uint32_t scratch[select_words(kChooseWarps)];
+  __shared__ __align__(16) uint32_t scratch[select_words(kChooseWarps)];
   if (a.cluster > 1) cluster_arrive();
   pdl_trigger();
   pdl_wait();
@@ -298,11 +346,13 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
         for (int i = 0; i < R::per_lane; ++i) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
       }
     };
+    fetch();           // on their way while the row's numbers are added up
     double u[R::values], d[R::values];
     const int group = a.q_heads / a.kv_heads;
     const typename L::type* q = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim);
 #pragma unroll
     for (int i = 0; i < R::values; ++i) u[i] = d[i] = 0;
+#pragma unroll 2
     for (int h = 0; h < group; ++h) {
 #pragma unroll
       for (int i = 0; i < R::per_lane; ++i) {
@@ -312,7 +362,6 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
         for (int x = 0; x < L::n; ++x) add_part(v[x], u[i * L::n + x], d[i * L::n + x]);
       }
     }
-    fetch();
     // the trip count is the same for all lanes: they exchange sums
     for (int base = from; base < seen; base += stride) {
       double sum[A];
@@ -383,7 +432,7 @@ template <typename T> __global__ void __launch_bounds__(kChooseThreads, 2) choos
   constexpr int kChunks = 2 * kDim / L::n, kSteps = kChunks / 4;        // 16-byte chunks of a page's bounds; those of one lane
   extern __shared__ double sums[];                       // [kSteps * L::n][row][lane of four]
   uint32_t* keys = reinterpret_cast<uint32_t*>(sums + 2 * kDim * kTileRows);   // [rows of this CTA][table_width]
-  __shared__ uint32_t scratch[kChooseWarps][select_words(1)];
+  __shared__ __align__(16) uint32_t scratch[kChooseWarps][select_words(1)];
   __shared__ int entries[kTileRows], seens[kTileRows];
   if (a.cluster > 1) cluster_arrive();
   pdl_trigger();

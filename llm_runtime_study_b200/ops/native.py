@@ -362,18 +362,32 @@ def require(t: torch.Tensor, name: str, *, dtype=None, shape=None, dims=None) ->
     return t
 
 
-def pointer(t: torch.Tensor, name: str, dtype: torch.dtype, *, shape: tuple | None = None, dims: int | None = None, align: int = 4) -> int:
-    """The address of an argument: a contiguous tensor of this type and shape on the current CUDA device, whose stream the kernels go
-    to, that starts on a multiple of ``align`` bytes.  (One pass over what a launch needs to know: a third of ``require``'s time.)"""
+def current_device() -> int:
+    """The current CUDA device; a number that no tensor's device has where there is none."""
 
-    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice() or t.dtype is not dtype or not t.is_contiguous()
-            or (shape is not None and t.shape != shape) or (dims is not None and t.dim() != dims)):
-        require(t, name, dtype=dtype, shape=shape, dims=dims)
-        raise KernelError(f"{name} is on {t.device}, but the current device is cuda:{torch._C._cuda_getDevice()}")
-    at = t.data_ptr()
-    if at % align:
-        raise KernelError(f"{name} must start on a multiple of {align} bytes")
-    return at
+    try:
+        return torch._C._cuda_getDevice()
+    except (AttributeError, RuntimeError):
+        return -2
+
+
+def pointer(t: torch.Tensor, name: str, here: int, dtype: torch.dtype, shape: tuple | None = None, dims: int | None = None,
+            align: int = 4) -> int:
+    """The address of an argument: a contiguous tensor of this type and shape on the device ``here`` (the current one, whose stream the
+    kernels go to), which starts on a multiple of ``align`` bytes.  (One pass over what a launch needs to know: the host is what bounds a
+    small launch.)"""
+
+    try:
+        if (t.get_device() == here and t.dtype is dtype and t.is_contiguous() and (shape is None or t.shape == shape)
+                and (dims is None or t.dim() == dims)):
+            at = t.data_ptr()
+            if at % align == 0:
+                return at
+            raise KernelError(f"{name} must start on a multiple of {align} bytes")
+    except AttributeError:        # no tensor
+        pass
+    require(t, name, dtype=dtype, shape=shape, dims=dims)
+    raise KernelError(f"{name} is on {t.device}, but the current device is cuda:{here}")
 
 
 def tag(dtype: torch.dtype) -> int:

@@ -35,10 +35,11 @@ class StepMaps:
 def page_table_set(tables: torch.Tensor, *, rows: torch.Tensor, columns: torch.Tensor, pages: torch.Tensor) -> None:
     """``tables[rows[i], columns[i]] = pages[i]`` (all int32, the cells distinct); a cell outside the table is left out."""
 
-    at = pointer(tables, "tables", torch.int32, dims=2)
-    rows_at = pointer(rows, "rows", torch.int32, dims=1)
+    here = native.current_device()
+    at = pointer(tables, "tables", here, torch.int32, dims=2)
+    rows_at = pointer(rows, "rows", here, torch.int32, dims=1)
     shape = rows.shape
-    columns_at, pages_at = pointer(columns, "columns", torch.int32, shape=shape), pointer(pages, "pages", torch.int32, shape=shape)
+    columns_at, pages_at = pointer(columns, "columns", here, torch.int32, shape=shape), pointer(pages, "pages", here, torch.int32, shape=shape)
     slots, width = tables.shape
     if not slots or not width:
         raise KernelError(f"a page table of shape {tuple(tables.shape)} has no cells")
@@ -58,10 +59,11 @@ def step_maps(
     ``out``: tensors to write into, which may have room for more entries and tokens than there are (those are left as they are);
     what is ``None`` there is not made."""
 
-    at = pointer(tables, "tables", torch.int32, dims=2)
-    slots_at = pointer(slots, "slots", torch.int32, dims=1)
+    here = native.current_device()
+    at = pointer(tables, "tables", here, torch.int32, dims=2)
+    slots_at = pointer(slots, "slots", here, torch.int32, dims=1)
     entries = slots.shape[0]
-    kv_len_at, counts_at = pointer(kv_len, "kv_len", torch.int32, shape=(entries,)), pointer(counts, "counts", torch.int32, shape=(entries,))
+    kv_len_at, counts_at = pointer(kv_len, "kv_len", here, torch.int32, shape=(entries,)), pointer(counts, "counts", here, torch.int32, shape=(entries,))
     table_rows, table_width = tables.shape
     if not table_rows or not table_width or page_size <= 0 or num_tokens < 0 or (width is not None and width <= 0):
         raise KernelError(f"tables {tuple(tables.shape)}, page_size {page_size}, num_tokens {num_tokens} and width {width} do not fit")
@@ -86,7 +88,7 @@ def step_maps(
             if t is None and dims == 1:
                 pointers.append(None)
                 continue
-            pointers.append(pointer(t, f"out.{name}", dtype, dims=dims, align=dtype.itemsize))
+            pointers.append(pointer(t, f"out.{name}", here, dtype, dims=dims, align=dtype.itemsize))
             if t.shape[0] < least:
                 raise KernelError(f"out.{name} has room for {t.shape[0]}, {least} are needed")
     if entries:
@@ -101,13 +103,14 @@ def slot_load_maps(records: torch.Tensor, slots: torch.Tensor, token_ids: torch.
     advance) and the batch's ``block_table`` from ``tables`` by those lengths, as ``step_maps`` makes it, in one launch.  The slots
     of live records are distinct."""
 
-    at = pointer(records, "records", torch.int32, dims=2)
+    here = native.current_device()
+    at = pointer(records, "records", here, torch.int32, dims=2)
     if records.shape[1] != SLOT_WORDS:
         raise KernelError(f"records of {records.shape[1]} words are not slot records")
     n = slots.shape[0]
-    given = [pointer(t, name, torch.int32, shape=(n,)) for t, name in ((slots, "slots"), (token_ids, "token_ids"), (positions, "positions"),
+    given = [pointer(t, name, here, torch.int32, shape=(n,)) for t, name in ((slots, "slots"), (token_ids, "token_ids"), (positions, "positions"),
                                                                      (kv_len, "kv_len"))]
-    tables_at, block_at = pointer(tables, "tables", torch.int32, dims=2), pointer(block_table, "block_table", torch.int32, dims=2)
+    tables_at, block_at = pointer(tables, "tables", here, torch.int32, dims=2), pointer(block_table, "block_table", here, torch.int32, dims=2)
     if tables.numel() == 0 or block_table.shape[0] < n or block_table.shape[1] == 0 or page_size <= 0:
         raise KernelError(f"tables {tuple(tables.shape)}, block_table {tuple(block_table.shape)} and page_size {page_size} do not fit {n} slots")
     native.call("b200_slot_load_maps", at, records.shape[0], *given, tables_at, tables.shape[0], tables.shape[1], block_at,

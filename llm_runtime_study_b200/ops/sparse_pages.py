@@ -22,7 +22,7 @@ _TABLE = {
     "b200_page_bounds": [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 6 + [c_void_p],
     "b200_choose_pages": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 11 + [c_void_p],
     "b200_choose_pages_tiles": [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 11 + [c_void_p],
-    "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p],
+    "b200_attend_chosen": [c_void_p] * 7 + [c_int, c_void_p] + [c_int] * 7 + [c_float, c_int, c_int, c_int, c_void_p],
 }
 SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
 DTYPES = (torch.float32, torch.bfloat16)
@@ -52,12 +52,12 @@ def build(head_dim: int) -> None:
     build_library(name, SOURCES, native.library_defines(name))
 
 
-def _pool(t: torch.Tensor, name: str) -> int:
+def _pool(t: torch.Tensor, name: str, here: int) -> int:
     """The address of pages of keys, which set the type of everything beside them."""
 
     if not isinstance(t, torch.Tensor) or t.dtype not in native.DTYPE_TAG:
         native.require(t, name, dtype=DTYPES)
-    return pointer(t, name, t.dtype, dims=4, align=16)
+    return pointer(t, name, here, t.dtype, dims=4, align=16)
 
 
 def _sizes(*sizes: int) -> None:
@@ -65,18 +65,18 @@ def _sizes(*sizes: int) -> None:
         raise KernelError(f"pages of sizes {sizes} hold nothing")
 
 
-def _rows(positions, token_entry, block_table, n: int) -> tuple[int, int, int, int]:
+def _rows(positions, token_entry, block_table, n: int, here: int) -> tuple[int, int, int, int]:
     """Addresses of the rows' positions and entries and of the block table, and the table's width."""
 
-    given = (pointer(positions, "positions", torch.int32, shape=(n,)), pointer(token_entry, "token_entry", torch.int32, shape=(n,)),
-             pointer(block_table, "block_table", torch.int32, dims=2), block_table.shape[1])
+    given = (pointer(positions, "positions", here, torch.int32, shape=(n,)), pointer(token_entry, "token_entry", here, torch.int32, shape=(n,)),
+             pointer(block_table, "block_table", here, torch.int32, dims=2), block_table.shape[1])
     if not block_table.numel():
         raise KernelError(f"a block table of shape {tuple(block_table.shape)} has no cells")
     return given
 
 
-def _query(q: torch.Tensor, kv_heads: int, head_dim: int, dtype) -> tuple[int, int, int]:
-    at = pointer(q, "q", dtype, dims=3, align=16)
+def _query(q: torch.Tensor, kv_heads: int, head_dim: int, dtype, here: int) -> tuple[int, int, int]:
+    at = pointer(q, "q", here, dtype, dims=3, align=16)
     n, heads, d = q.shape
     if d != head_dim or heads == 0 or heads % kv_heads:
         raise KernelError(f"q {tuple(q.shape)} does not fit {kv_heads} key heads of {head_dim}")
@@ -92,15 +92,16 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
     ``[pages, kv heads, 2, d]`` (low, high) of the same type; ``max_q_len``: the most new tokens of an entry (a hint for the
     launch).  Pages that are not full keep what they have; a NaN among a channel's keys makes both bounds NaN."""
 
-    at = _pool(keys, "keys")
+    here = native.current_device()
+    at = _pool(keys, "keys", here)
     pages, kv_heads, page_size, d = keys.shape
     library = library_name(d)
     _sizes(pages, kv_heads, page_size)
-    bounds_at = pointer(bounds, "bounds", keys.dtype, shape=(pages, kv_heads, 2, d), align=16)
-    kv_len_at = pointer(kv_len, "kv_len", torch.int32, dims=1)
+    bounds_at = pointer(bounds, "bounds", here, keys.dtype, shape=(pages, kv_heads, 2, d), align=16)
+    kv_len_at = pointer(kv_len, "kv_len", here, torch.int32, dims=1)
     entries = kv_len.shape[0]
-    q_start_at = pointer(q_start, "q_start", torch.int32, shape=(entries + 1,))
-    table_at = pointer(block_table, "block_table", torch.int32, dims=2)
+    q_start_at = pointer(q_start, "q_start", here, torch.int32, shape=(entries + 1,))
+    table_at = pointer(block_table, "block_table", here, torch.int32, dims=2)
     rows, width = block_table.shape
     if rows != entries or (entries and not width):
         raise KernelError(f"a block table of shape {tuple(block_table.shape)} does not fit {entries} entries")
@@ -112,7 +113,7 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
 
 
 @lru_cache(maxsize=4096)
-def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[int, int]:
+def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[bool, int]:
     """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each; a cluster shares out
     the pages of a row or a tile where there are few of them (bfloat16, 40 heads over 8 of 128, pages of 32, 65,521 tokens, clusters of
     1, 2, 4 and 8: 1 request 35, 22, 15 and 12 us, 8 requests 35, 23, 18 and 23, 32 requests 53, 52, 62 and 84), and the shared memory
@@ -142,14 +143,15 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
     taken, a NaN (an infinite bound that meets a sum of 0 gives one) ranks first.  A page that is not held (an id that is none) is
     not chosen."""
 
-    at = _pool(bounds, "bounds")
+    here = native.current_device()
+    at = _pool(bounds, "bounds", here)
     pages, kv_heads, two, d = bounds.shape
     library = library_name(d)
     _sizes(pages, kv_heads)
     if two != 2:
         raise KernelError(f"bounds of shape {tuple(bounds.shape)} are not [pages, kv heads, 2, d]")
-    q_at, n, heads = _query(q, kv_heads, d, bounds.dtype)
-    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n)
+    q_at, n, heads = _query(q, kv_heads, d, bounds.dtype, here)
+    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n, here)
     if page_size <= 0 or first < 0 or last < 1 or budget < first + last:
         raise KernelError(f"page_size {page_size}, budget {budget}, first {first} and last {last}: the budget holds the first pages and "
                           "the last ones, of which there is one at least")
@@ -168,19 +170,22 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
 
 
 @lru_cache(maxsize=4096)
-def attention_parts(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> int:
-    """Into how many CTAs of a cluster the list of a row and kv head is cut: 1, 2, 4 or 8.  float32: from the list's length alone, so
-    that the order of the sums does not depend on the batch.  bfloat16: until the GPU is full, no part shorter than 128 keys."""
+def attention_shape(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> tuple[int, bool]:
+    """(CTAs of a cluster that the list of a row and kv head is cut over: 1, 2, 4 or 8; twice the warps a CTA).  No
+    part is shorter than 128 keys.  float32: from the list's length alone, so that the order of the sums does not depend on the batch.
+    bfloat16: until the GPU is full (32 heads over 8 of 128, 2,048 keys a row, 1, 2, 4 and 8 parts: 1 request 47, 26, 15 and 11 us, 16
+    requests 65, 39, 28 and 33, 64 requests of 64 heads 88, 98, 108 and 129), and eight warps to a CTA instead of four as long as
+    every CTA has a multiprocessor of its own (1 request 7.8 us instead of 10.6)."""
 
     keys, parts = budget * page_size, 1
     if dtype == torch.float32:
-        while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 256:
+        while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128:
             parts *= 2
-        return parts
+        return parts, False
     ctas = rows * kv_heads * -(-(heads // kv_heads) // 8)
     while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128 and 2 * parts * ctas <= 2 * native.sm_count():
         parts *= 2
-    return parts
+    return parts, ctas * parts <= native.sm_count()
 
 
 def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, chosen: torch.Tensor, *, positions: torch.Tensor,
@@ -190,14 +195,15 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     ``values`` are ``[pages, kv heads, page size, d]``.  Keys behind the position and pages that are not held are neither read nor
     counted; a row without a key (or without a score above minus infinity) gives zeros."""
 
-    at = _pool(keys, "keys")
+    here = native.current_device()
+    at = _pool(keys, "keys", here)
     pages, kv_heads, page_size, d = shape = keys.shape
     library = library_name(d)
     _sizes(pages, kv_heads, page_size)
-    values_at = pointer(values, "values", keys.dtype, shape=shape, align=16)
-    q_at, n, heads = _query(q, kv_heads, d, keys.dtype)
-    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n)
-    chosen_at = pointer(chosen, "chosen", torch.int32, dims=3)
+    values_at = pointer(values, "values", here, keys.dtype, shape=shape, align=16)
+    q_at, n, heads = _query(q, kv_heads, d, keys.dtype, here)
+    positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n, here)
+    chosen_at = pointer(chosen, "chosen", here, torch.int32, dims=3)
     rows, of_heads, budget = chosen.shape
     if rows != n or of_heads != kv_heads or not budget:
         raise KernelError(f"chosen of shape {tuple(chosen.shape)} does not fit {n} rows of {kv_heads} key heads")
@@ -207,6 +213,6 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     if n:
         native.call("b200_attend_chosen", q_at, at, values_at, chosen_at, positions_at, entry_at, table_at, width, out.data_ptr(), n,
                     block_table.shape[0], heads, kv_heads, page_size, pages, budget, float(scale),
-                    attention_parts(n, heads, kv_heads, budget, page_size, keys.dtype), native.DTYPE_TAG[keys.dtype], stream_ptr(),
+                    *attention_shape(n, heads, kv_heads, budget, page_size, keys.dtype), native.DTYPE_TAG[keys.dtype], stream_ptr(),
                     library=library)
     return out

@@ -14,7 +14,7 @@ from tests.plain import sparse_pages_plain as plain
 def host(monkeypatch):
     """The operators with CPU tensors taken for CUDA ones; a launch is an error of the test."""
 
-    def pointer(t, name, dtype, *, shape=None, dims=None, align=4):
+    def pointer(t, name, here, dtype, shape=None, dims=None, align=4):
         if t.dtype is not dtype or not t.is_contiguous() or (shape is not None and t.shape != shape) or (dims is not None and t.dim() != dims):
             raise KernelError(name)
         if t.data_ptr() % align:
@@ -163,7 +163,7 @@ def test_cpu_tensors_are_refused():
         page_tables.step_maps(ints(3, 4), slots=ints(1), kv_len=ints(1), counts=ints(1), page_size=8, num_tokens=1)
 
 
-def test_tensors_of_another_device_are_refused(monkeypatch):
+def test_tensors_of_another_device_are_refused():
     class Elsewhere(torch.Tensor):
         is_cuda, index = True, 1
         device = torch.device("cuda", 1)
@@ -172,18 +172,20 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
             return self.index
 
     t = torch.zeros(64, dtype=torch.int32).as_subclass(Elsewhere)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     with pytest.raises(KernelError, match="current device"):
-        native.pointer(t, "q", torch.int32)
+        native.pointer(t, "q", 0, torch.int32)
     Elsewhere.index = 0
-    assert native.pointer(t, "q", torch.int32, shape=(64,), dims=1) == t.data_ptr()
+    assert native.pointer(t, "q", 0, torch.int32, shape=(64,), dims=1) == t.data_ptr()
     for wrong in (dict(shape=(63,)), dict(dims=2)):
         with pytest.raises(KernelError):
-            native.pointer(t, "q", torch.int32, **wrong)
+            native.pointer(t, "q", 0, torch.int32, **wrong)
+    for wrong in (None, 7, "q"):
+        with pytest.raises(KernelError, match="CUDA"):
+            native.pointer(wrong, "q", 0, torch.int32)
     with pytest.raises(KernelError, match="dtype"):
-        native.pointer(t, "q", torch.int64)
+        native.pointer(t, "q", 0, torch.int64)
     with pytest.raises(KernelError, match="multiple"):
-        native.pointer(t[1:], "q", torch.int32, align=16)
+        native.pointer(t[1:], "q", 0, torch.int32, align=16)
 
 
 def test_a_page_s_score_bounds_the_scores_of_its_keys():

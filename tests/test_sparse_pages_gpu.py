@@ -212,6 +212,32 @@ def test_equal_scores_go_to_the_lower_page(dtype, rows):
     assert torch.equal(cache.plain_choose(9, 1, 2), got)
 
 
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_that_differ_in_their_last_bits(dtype, d, rows):
+    """Pages alike but for one small channel, one step up or down: scores a few float32 steps apart, or equal."""
+
+    cache = Cache([600], [rows], heads=4, kv_heads=2, d=d, page=4, dtype=dtype, seed=d)
+    g = torch.Generator().manual_seed(5)
+    cache.bounds[:] = cache.bounds[0]
+    channel = int(cache.q[0].float().abs().sum(0).argmin())
+    step = torch.finfo(dtype).eps * torch.randint(-3, 4, (cache.bounds.shape[0], 2, 2), generator=g)
+    cache.bounds[..., channel] = (cache.bounds[..., channel].float() * (1 + step)).to(dtype)
+    for budget in (5, 20, 75):
+        assert torch.equal(cache.choose(budget, 1, 2).cpu(), cache.plain_choose(budget, 1, 2))
+
+
+@pytest.mark.parametrize("rows", [1, 10])
+@pytest.mark.parametrize("q_scale,bound_scale", [(1e-30, 1.0), (1e-36, 1e-5), (1e-38, 1e30), (1e30, 1e-30), (1e18, 1e18), (1.0, 1e38), (0.0, 1.0), (1.0, 1e-39)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_very_small_and_very_large_numbers(dtype, q_scale, bound_scale, rows):
+    cache = Cache([300], [rows], heads=4, kv_heads=2, d=32, page=4, dtype=dtype)
+    cache.q = (cache.q.double() * q_scale).to(dtype)
+    cache.bounds = (cache.bounds.double() * bound_scale).to(dtype)
+    assert torch.equal(cache.choose(20, 1, 2).cpu(), cache.plain_choose(20, 1, 2))
+
+
 @pytest.mark.parametrize("rows", [1, 9])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_nan_ranks_first_and_infinities_keep_their_order(dtype, rows):
