@@ -252,21 +252,28 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   return r;
 }
 
+// 2^x of a weight that is rounded to bfloat16 next: to 22 bits, results below 2^-126 as 0.
+__device__ __forceinline__ float power_of_two(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+
 constexpr int kRowRegs = kDim / 8;              // registers of a lane for its channels of one row: pairs
 constexpr int kTiles = kDim / 16;                // tiles of 16 value columns
 constexpr bool kSwapOdd = kDim % 64 == 0;       // rows of whole 128 bytes
 
-// A lane's channels of one row: 8 t .. 8 t + 7 of every 32, 4 t .. 4 t + 3 of the last 16.
-__device__ __forceinline__ void load_channels(uint32_t (&r)[kRowRegs], const __nv_bfloat16* row, int t, bool odd, bool is) {
+// A lane's channels of one row: 8 t .. 8 t + 7 of every 32, 4 t .. 4 t + 3 of the last 16.  ALL: the row is one to read.
+template <bool ALL> __device__ __forceinline__ void load_channels(uint32_t (&r)[kRowRegs], const __nv_bfloat16* row, int t, bool odd, bool is) {
 #pragma unroll
   for (int b = 0; b < kDim / 32; ++b) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (is) v = load_row_16(row + 32 * (kSwapOdd && odd ? b ^ 1 : b) + 8 * t);
+    if (ALL || is) v = load_row_16(row + 32 * (kSwapOdd && odd ? b ^ 1 : b) + 8 * t);
     r[4 * b] = v.x, r[4 * b + 1] = v.y, r[4 * b + 2] = v.z, r[4 * b + 3] = v.w;
   }
   if (kDim % 32) {
     uint2 v = make_uint2(0, 0);
-    if (is) v = load_row_8(row + kDim / 32 * 32 + 4 * t);
+    if (ALL || is) v = load_row_8(row + kDim / 32 * 32 + 4 * t);
     r[kRowRegs - 2] = v.x, r[kRowRegs - 1] = v.y;
   }
 }
@@ -290,7 +297,7 @@ __device__ __forceinline__ int column_of(int m, int half, int g) {
 
 // NT: tiles of eight query heads of a CTA.  WHOLE: pages are whole tiles of 16 keys, so that a tile is a run of rows.
 template <int NT, int WARPS, bool WHOLE>
-__global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 && kDim <= 128 ? 16 / WARPS : 1) attend_mma_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int H = 8 * NT;
   __shared__ float sums[WARPS][H][kSumsRow];
   __shared__ float top[WARPS][H], total[WARPS][H];
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
   const size_t q_row = (static_cast<size_t>(w.row) * a.q_heads + w.head * group + w.slice * H) * kDim;
   uint32_t q[NT][kRowRegs];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) load_channels(q[n], static_cast<const __nv_bfloat16*>(a.q) + q_row + (8 * n + g) * kDim, t, false, 8 * n + g < heads_here);
+  for (int n = 0; n < NT; ++n) load_channels<false>(q[n], static_cast<const __nv_bfloat16*>(a.q) + q_row + (8 * n + g) * kDim, t, false, 8 * n + g < heads_here);
   float o[NT][kTiles][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -343,10 +350,17 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
         }
       }
       uint32_t k0[kRowRegs], k1[kRowRegs], v0[kRowRegs], v1[kRowRegs];
-      load_channels(k0, keys + at[0], t, odd, is[0]);
-      load_channels(k1, keys + at[1], t, odd, is[1]);
-      load_channels(v0, values + at[0], t, odd, is[0]);
-      load_channels(v1, values + at[1], t, odd, is[1]);
+      if (__all_sync(0xffffffffu, is[0] && is[1])) {        // most tiles: nothing to blank out
+        load_channels<true>(k0, keys + at[0], t, odd, true);
+        load_channels<true>(k1, keys + at[1], t, odd, true);
+        load_channels<true>(v0, values + at[0], t, odd, true);
+        load_channels<true>(v1, values + at[1], t, odd, true);
+      } else {
+        load_channels<false>(k0, keys + at[0], t, odd, is[0]);
+        load_channels<false>(k1, keys + at[1], t, odd, is[1]);
+        load_channels<false>(v0, values + at[0], t, odd, is[0]);
+        load_channels<false>(v1, values + at[1], t, odd, is[1]);
+      }
       order_channels(k0, odd);
       order_channels(k1, odd);
       uint32_t weights[NT][2];
@@ -366,9 +380,9 @@ __global__ void __launch_bounds__(WARPS * 32) attend_mma_kernel(const __grid_con
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
           most = fmaxf(most, m[n][c]);
           const float base = most == -CUDART_INF_F ? 0.f : most;
-          keep[c] = exp2f(m[n][c] - base);
+          keep[c] = power_of_two(m[n][c] - base);
           m[n][c] = most;
-          x = exp2f(x - base), y = exp2f(y - base);
+          x = power_of_two(x - base), y = power_of_two(y - base);
           l[n][c] = l[n][c] * keep[c] + x + y;
           s[0][c] = x, s[0][2 + c] = y;
         }
