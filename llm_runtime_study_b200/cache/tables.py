@@ -32,7 +32,7 @@ class DeviceTables:
         self._known: dict[int, _Known] = {}
 
     def changes(self, requests: Sequence) -> list[np.ndarray]:
-        """Per group: the cells that differ from what the device holds, int32 ``[3, cells]`` (row, column, page)."""
+        """The cells that differ from what the device holds: for every group their rows, columns and pages (int32)."""
 
         groups = len(self.tensors)
         rows: list[list[int]] = [[] for _ in range(groups)]
@@ -54,7 +54,7 @@ class DeviceTables:
                     pages[g].append(-1)
                     back += 1
                 rows[g].extend([request.slot] * (len(columns[g]) - len(rows[g])))
-        return [np.asarray([rows[g], columns[g], pages[g]], dtype=np.int32) for g in range(groups)]
+        return [np.asarray(cells[g], dtype=np.int32) for g in range(groups) for cells in (rows, columns, pages)]
 
     def sent(self, requests: Sequence) -> None:
         """The changes of these requests are on their way to the device, before everything that is launched from now on."""

@@ -112,8 +112,8 @@ class DecodeGraph:
         runner, manager = self.runner, self.runner.manager
         if manager.tables is not None:
             changes = manager.tables.changes(requests)
-            if any(cells.shape[1] for cells in changes):
-                runner.set_tables(requests, changes, runner._send(changes))
+            if any(cells.size for cells in changes):
+                runner.set_tables(requests, runner._send(changes))
         sent = np.zeros(self.sent, dtype=np.int32)
         sent[:b] = manager.padding_slot
         sent[: len(requests)] = [r.slot for r in requests]

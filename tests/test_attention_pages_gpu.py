@@ -115,11 +115,14 @@ def test_portions_batches_and_new_pages_do_not_change_a_bit(tmp_path):
     assert torch.equal(torch.cat(logits), want)
 
 
+@pytest.mark.parametrize("least", [0, 10 ** 6])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_captured_decode_equals_eager(tmp_path, dtype):
+def test_captured_decode_equals_eager(tmp_path, monkeypatch, dtype, least):
     from tests.test_generate_gpu import _decode_both_ways
+    from llm_runtime_study_b200.engine import step
     from llm_runtime_study_b200.sampling import SamplingConfig
 
+    monkeypatch.setattr(step, "DEVICE_TABLES_MIN_PAGES", least)      # eager steps with tables made on the device, or by the host
     loaded, raw, _, page = _load(tmp_path, "B", dtype, 3)
     rng = random.Random(6)
     prompts = [helpers.random_tokens(rng, raw["vocab_size"], n) for n in (3, 70, 9, 41)]
@@ -187,15 +190,18 @@ class _Nothing:
         return None
 
 
-@pytest.mark.parametrize("seed", range(4))
-def test_tables_on_the_device_follow_the_host_s(seed):
-    """Random steps over three groups of pages (a window, a page size of its own): admission, portions, decoding, roll-backs,
+@pytest.mark.parametrize("least", [0, 40, 10 ** 6])
+@pytest.mark.parametrize("seed", range(3))
+def test_tables_on_the_device_follow_the_host_s(monkeypatch, seed, least):
+    """(``least``: pages from which a step's tables are made on the device; all of them, some, none.)  Random steps over three groups of pages (a window, a page size of its own): admission, portions, decoding, roll-backs,
     release and reuse of slots; block tables, positions and slot maps equal what the host's tables say."""
 
     from llm_runtime_study_b200.cache.manager import CacheLayout, CacheManager
     from llm_runtime_study_b200.engine.step import StepEntry, StepRunner
+    from llm_runtime_study_b200.engine import step
     from llm_runtime_study_b200.parts.base import PagedKV, Runtime
 
+    monkeypatch.setattr(step, "DEVICE_TABLES_MIN_PAGES", least)
     rng = random.Random(seed)
     layout = CacheLayout.from_requirements([PagedKV(1, 16), PagedKV(1, 16, window=9), PagedKV(1, 16, page_size=5)])
     device = torch.device("cuda:0")
@@ -225,7 +231,9 @@ def test_tables_on_the_device_follow_the_host_s(seed):
                 table = entry.request.tables[g]
                 held = table[: -(-length // pool.page_size)]
                 row = ctx.block_table(g)[i].tolist()
-                assert row == held + [-1] * (len(row) - len(held)), (g, i)
+                # behind its last page a row ends; one put together by the host shows pages taken in advance, too
+                rest = [-1] * (len(row) - len(held)) if least == 0 else (table[len(held) :] + [-1] * len(row))[: len(row) - len(held)]
+                assert row[: len(held)] == held and (row[len(held) :] == rest or set(row[len(held) :]) <= {-1}), (g, i)
                 want = [table[p // pool.page_size] * pool.page_size + p % pool.page_size for p in range(length - n, length)]
                 assert ctx.slot_map(g)[at : at + n].tolist() == want
             at += n
