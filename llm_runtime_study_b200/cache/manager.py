@@ -131,7 +131,8 @@ class GroupPool:
         })
         self.allocator = PageAllocator(num_pages)
         elements = sum(int(torch.tensor(shape).prod()) for _, shape in group.requirement.tensors)
-        self.bytes_per_token = len(group.layers) * elements * torch.empty((), dtype=dtype).element_size()
+        per_page = sum(int(torch.tensor(shape).prod()) for _, shape in group.requirement.page_tensors)
+        self.bytes_per_token = len(group.layers) * (elements + -(-per_page // page_size)) * torch.empty((), dtype=dtype).element_size()
 
     def pages_for(self, tokens: int) -> int:
         return -(-tokens // self.page_size)

@@ -65,7 +65,8 @@ def step_maps(
     entries = slots.shape[0]
     kv_len_at, counts_at = pointer(kv_len, "kv_len", here, torch.int32, shape=(entries,)), pointer(counts, "counts", here, torch.int32, shape=(entries,))
     table_rows, table_width = tables.shape
-    if not table_rows or not table_width or page_size <= 0 or num_tokens < 0 or (width is not None and width <= 0):
+    if (not table_rows or not table_width or not 0 < page_size < 1 << 31 or not 0 <= num_tokens < 1 << 31
+            or (width is not None and not 0 < width < 1 << 31)):
         raise KernelError(f"tables {tuple(tables.shape)}, page_size {page_size}, num_tokens {num_tokens} and width {width} do not fit")
     if out is None:
         device = tables.device
@@ -111,7 +112,7 @@ def slot_load_maps(records: torch.Tensor, slots: torch.Tensor, token_ids: torch.
     given = [pointer(t, name, here, torch.int32, shape=(n,)) for t, name in ((slots, "slots"), (token_ids, "token_ids"), (positions, "positions"),
                                                                      (kv_len, "kv_len"))]
     tables_at, block_at = pointer(tables, "tables", here, torch.int32, dims=2), pointer(block_table, "block_table", here, torch.int32, dims=2)
-    if tables.numel() == 0 or block_table.shape[0] < n or block_table.shape[1] == 0 or page_size <= 0:
+    if tables.numel() == 0 or block_table.shape[0] < n or block_table.shape[1] == 0 or not 0 < page_size < 1 << 31:
         raise KernelError(f"tables {tuple(tables.shape)}, block_table {tuple(block_table.shape)} and page_size {page_size} do not fit {n} slots")
     native.call("b200_slot_load_maps", at, records.shape[0], *given, tables_at, tables.shape[0], tables.shape[1], block_at,
                 block_table.shape[1], n, int(page_size), native.stream_ptr())

@@ -26,6 +26,7 @@ _TABLE = {
 }
 SOURCES = ("sparse_pages.cu", "sparse_attention.cu")
 DTYPES = (torch.float32, torch.bfloat16)
+MAX_SIZE = 1 << 30           # of a page or a list
 MAX_TABLE_WIDTH = 51200      # pages of a row whose scores fit into a CTA's shared memory
 
 
@@ -108,7 +109,7 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
     if max_q_len < 0:
         raise KernelError("max_q_len must not be negative")
     if entries and max_q_len:
-        native.call("b200_page_bounds", at, bounds_at, table_at, width, q_start_at, kv_len_at, entries, -(-max_q_len // page_size), kv_heads,
+        native.call("b200_page_bounds", at, bounds_at, table_at, width, q_start_at, kv_len_at, entries, min(-(-max_q_len // page_size), width), kv_heads,
                     page_size, pages, native.DTYPE_TAG[keys.dtype], stream_ptr(), library=library)
 
 
@@ -152,13 +153,11 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
         raise KernelError(f"bounds of shape {tuple(bounds.shape)} are not [pages, kv heads, 2, d]")
     q_at, n, heads = _query(q, kv_heads, d, bounds.dtype, here)
     positions_at, entry_at, table_at, width = _rows(positions, token_entry, block_table, n, here)
-    if page_size <= 0 or first < 0 or last < 1 or budget < first + last:
+    if not 0 < page_size <= MAX_SIZE or first < 0 or last < 1 or not first + last <= budget <= MAX_SIZE:
         raise KernelError(f"page_size {page_size}, budget {budget}, first {first} and last {last}: the budget holds the first pages and "
                           "the last ones, of which there is one at least")
     if width > MAX_TABLE_WIDTH:
         raise KernelError(f"block tables of more than {MAX_TABLE_WIDTH} pages are not taken: {width}")
-    if n * kv_heads * budget >= 1 << 40:
-        raise KernelError(f"a budget of {budget} pages for {n} rows of {kv_heads} heads is too much")
     chosen = torch.empty((n, kv_heads, budget), dtype=torch.int32, device=q.device)
     if n:
         entries = block_table.shape[0]
@@ -207,7 +206,7 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     rows, of_heads, budget = chosen.shape
     if rows != n or of_heads != kv_heads or not budget:
         raise KernelError(f"chosen of shape {tuple(chosen.shape)} does not fit {n} rows of {kv_heads} key heads")
-    if budget * page_size > 1 << 30:
+    if budget * page_size > MAX_SIZE:
         raise KernelError(f"{budget} pages of {page_size} tokens a row are too many")
     out = torch.empty_like(q)
     if n:

@@ -179,6 +179,38 @@ def test_what_the_engine_refuses(tmp_path):
         Engine.from_random_weights(helpers.SORULIX_A, device="cuda:0", dtype="float32", max_seq_len=32, attention_pages=8)
 
 
+def test_the_command_line_takes_the_option(tmp_path):
+    import io
+
+    from llm_runtime_study_b200.cli import main
+
+    raw, seed, page = helpers.TINY["A"]
+    path, weights = helpers.make_model_dir(tmp_path / "m", raw, seed)
+    prompt = " ".join(str(t) for t in helpers.random_tokens(random.Random(1), raw["vocab_size"], 70))
+    texts = []
+    for pages in ("3", "64"):
+        out, err = io.StringIO(), io.StringIO()
+        options = ["--model", str(path), "--prompt-ids", prompt, "--max-new-tokens", "12", "--dtype", "float32", "--page-size", str(page),
+                   "--max-seq-len", "128", "--no-metrics"]
+        assert main([*options, "--attention-pages", pages], output=out, error=err) == 0, err.getvalue()
+        texts.append(out.getvalue())
+        assert main([*options, "--attention-pages", "2"], output=out, error=err) == 2 and "attention_pages" in err.getvalue()
+    out = io.StringIO()
+    assert main(options, output=out, error=io.StringIO()) == 0
+    assert texts[1] == out.getvalue() and texts[0].split()       # a budget of all pages reads them all
+
+
+def test_the_cache_counts_what_it_keeps_per_page():
+    from llm_runtime_study_b200.cache.manager import CacheLayout, CacheManager
+    from llm_runtime_study_b200.parts.base import PagedKV
+
+    plain, kept = (CacheManager(CacheLayout.from_requirements([PagedKV(2, 16, page_tensors=t)] * 3), max_tokens=64, page_size=8, max_requests=2,
+                                dtype=torch.bfloat16, device="cuda") for t in ((), (("bounds", (2, 2, 16)),)))
+    assert kept.groups[0].tensors["bounds"].shape == (3, 8, 2, 2, 16) and kept.layer_cache(1).tensors["bounds"].shape == (8, 2, 2, 16)
+    assert kept.num_bytes - plain.num_bytes == 3 * 8 * 64 * 2
+    assert kept.bytes_per_token() - plain.bytes_per_token() == 3 * 8 * 2
+
+
 # ------------------------------------------------------------------------------------------------ tables on the device
 class _Nothing:
     """A model of no layers, for the runner's bookkeeping."""

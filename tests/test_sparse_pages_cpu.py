@@ -101,6 +101,8 @@ REFUSED = [
     (_choose, dict(block_table=ints(0, 9))),
     (_choose, dict(block_table=ints(2, sparse_pages.MAX_TABLE_WIDTH + 1))),
     (_choose, dict(page_size=0)),
+    (_choose, dict(page_size=(1 << 32) + 16)),
+    (_choose, dict(budget=1 << 31)),
     (_choose, dict(budget=1)),
     (_choose, dict(budget=3, first=2, last=2)),
     (_choose, dict(last=0)),
@@ -137,7 +139,8 @@ def test_page_tables_refuse_what_does_not_fit(host):
     host.clear()
     made = page_tables.StepMaps(ints(2, 4), ints(3), ints(4), ints(4), ints(4).long())
     for change in (dict(tables=ints(3)), dict(tables=ints(0, 4)), dict(tables=tables.long()), dict(slots=ints(3)), dict(counts=ints(1)),
-                   dict(kv_len=ints(2).long()), dict(page_size=0), dict(num_tokens=-1), dict(width=0), dict(width=3, out=made),
+                   dict(kv_len=ints(2).long()), dict(page_size=0), dict(page_size=(1 << 32) + 8), dict(num_tokens=1 << 32), dict(width=1 << 32),
+                   dict(num_tokens=-1), dict(width=0), dict(width=3, out=made),
                    dict(num_tokens=5, out=made), dict(tables=ints(4, 3).T)):
         with pytest.raises(KernelError):
             maps(**change)
