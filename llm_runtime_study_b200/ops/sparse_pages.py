@@ -115,23 +115,25 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
 
 @lru_cache(maxsize=4096)
 def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[bool, int]:
-    """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each; a cluster shares out
-    the pages of a row or a tile where there are few of them (bfloat16, 40 heads over 8 of 128, pages of 32, 65,521 tokens, clusters of
-    1, 2, 4 and 8: 1 request 35, 22, 15 and 12 us, 8 requests 35, 23, 18 and 23, 32 requests 53, 52, 62 and 84), and the shared memory
-    that the scores of many pages need."""
+    """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each, in clusters where the
+    scores of many pages want the shared memory or few tiles would not fill the GPU.  For single tokens as many CTAs as let two a
+    multiprocessor be there at once, three where each would still have 512 pages (bfloat16, 32 heads over 8 of 128, clusters of 1, 2, 4
+    and 8; 2,048 pages: 1 request 34.5, 21.5, 14.6 and 11.0 us, 8 requests 34.8, 21.9, 17.0 and 22.4, 24 requests 51.6, 41.4, 44.9 and
+    59.0, 64 requests 79, 91, 109 and 145; 512 pages: 1 request 12.4, 9.5, 7.8 and 6.7, 24 requests 14.3, 18.5, 21.7 and 33.3)."""
 
-    def fill(units: int, cluster: int) -> int:
-        while cluster < 8 and 2 * cluster * units <= 2 * native.sm_count() and width // (2 * cluster) >= 64:
-            cluster *= 2
-        return cluster
-
+    sms = native.sm_count()
     if rows >= 2 * entries:
-        sums, cluster = 2 * head_dim * 64, 1
+        units, sums, cluster = -(-rows // 8) * kv_heads, 2 * head_dim * 64, 1
         while cluster < 8 and sums + 32 * width // cluster > 100 * 1024:
             cluster *= 2
+        while cluster < 8 and 2 * cluster * units <= 2 * sms and width // (2 * cluster) >= 64:
+            cluster *= 2
         if sums + 32 * width // cluster <= 200 * 1024:
-            return True, fill(-(-rows // 8) * kv_heads, cluster)
-    return False, fill(rows * kv_heads, 1)
+            return True, cluster
+    units, cluster = rows * kv_heads, 1
+    while cluster < 8 and width // (2 * cluster) >= 64 and 2 * cluster * units <= (3 if width // (2 * cluster) >= 512 else 2) * sms:
+        cluster *= 2
+    return False, cluster
 
 
 def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tensor, token_entry: torch.Tensor, block_table: torch.Tensor,
@@ -170,11 +172,11 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
 
 @lru_cache(maxsize=4096)
 def attention_shape(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> tuple[int, bool]:
-    """(CTAs of a cluster that the list of a row and kv head is cut over: 1, 2, 4 or 8; twice the warps a CTA).  No
-    part is shorter than 128 keys.  float32: from the list's length alone, so that the order of the sums does not depend on the batch.
-    bfloat16: until the GPU is full (32 heads over 8 of 128, 2,048 keys a row, 1, 2, 4 and 8 parts: 1 request 47, 26, 15 and 11 us, 16
-    requests 65, 39, 28 and 33, 64 requests of 64 heads 88, 98, 108 and 129), and eight warps to a CTA instead of four as long as
-    every CTA has a multiprocessor of its own (1 request 7.8 us instead of 10.6)."""
+    """(CTAs of a cluster that the list of a row and kv head is cut over: 1, 2, 4 or 8; twice the warps a CTA).  No part is shorter than
+    128 keys.  float32: from the list's length alone, so that the order of the sums does not depend on the batch.  bfloat16: as many
+    parts as let two CTAs of eight warps a multiprocessor be there at once; CTAs of four warps where there are more rows than that (32
+    heads over 8 of 128, 2,048 keys a row, parts and "w" for eight warps: 1 request 8: 8.5, 8w: 7.8 us; 8 requests 8: 16.7, 4w: 16.4; 16
+    requests 2: 30.4, 4: 26.8, 1w: 29.0, 2w: 26.6; 32 requests 1: 51.6, 2: 48.5, 1w: 46.1, 2w: 51.1; 40 requests 1: 64, 1w: 72, 2w: 72)."""
 
     keys, parts = budget * page_size, 1
     if dtype == torch.float32:
@@ -184,7 +186,7 @@ def attention_shape(rows: int, heads: int, kv_heads: int, budget: int, page_size
     ctas = rows * kv_heads * -(-(heads // kv_heads) // 8)
     while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128 and 2 * parts * ctas <= 2 * native.sm_count():
         parts *= 2
-    return parts, ctas * parts <= native.sm_count()
+    return parts, ctas * parts <= 2 * native.sm_count()
 
 
 def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, chosen: torch.Tensor, *, positions: torch.Tensor,

@@ -210,3 +210,25 @@ def test_plain_choice_keeps_the_first_and_the_last_pages():
     at = torch.tensor([70]), torch.tensor([0])
     assert plain.choose_pages(q, bounds, *at, table, 8, 4, 1, 2).tolist() == [[[0, 4, 7, 8]]]
     assert plain.choose_pages(q, bounds, *at, table, 8, 5, 1, 2).tolist() == [[[0, 1, 4, 7, 8]]]
+
+
+def test_shapes_of_the_launches():
+    """On a B200's 148 multiprocessors (what the rules assume where no device is visible)."""
+
+    shape = lambda *a: sparse_pages.choose_shape.__wrapped__(*a)      # noqa: E731
+    assert [shape(n, n, 8, 2048, 128) for n in (1, 8, 16, 24, 64)] == [(False, c) for c in (8, 4, 2, 2, 1)]
+    assert [shape(n, n, 8, 512, 128) for n in (1, 24)] == [(False, 8), (False, 1)]
+    assert shape(1, 1, 1, 4, 64) == (False, 1)
+    assert shape(500, 2, 8, 1024, 128) == (True, 1) and shape(8, 1, 1, 1024, 128) == (True, 8)
+    assert shape(500, 2, 8, 8192, 128)[0] and shape(500, 2, 8, 8192, 128)[1] >= 4       # scores of many pages lie in several CTAs
+    for width in (1, 100, 3000, 20000, sparse_pages.MAX_TABLE_WIDTH):                    # and what is chosen fits
+        for d in (16, 128, 256):
+            for rows, entries in ((1, 1), (40, 1), (40, 40)):
+                tiles, cluster = shape(rows, entries, 8, width, d)
+                assert cluster in (1, 2, 4, 8)
+                assert (width * (8 // cluster) * 4 + 2 * d * 64 if tiles else width * 4) <= 200 * 1024
+    attend = lambda *a: sparse_pages.attention_shape.__wrapped__(*a)      # noqa: E731
+    bf16, f32 = torch.bfloat16, torch.float32
+    assert [attend(n, 32, 8, 128, 16, bf16) for n in (1, 8, 16, 24, 40)] == [(8, True), (4, True), (2, True), (1, True), (1, False)]
+    assert attend(1, 32, 8, 4, 16, bf16) == (1, True) and attend(1, 8, 8, 1, 4096, bf16) == (1, True)      # one page is one part
+    assert attend(1, 32, 8, 128, 16, f32) == attend(4000, 32, 8, 128, 16, f32) == (8, False)               # the list alone decides
