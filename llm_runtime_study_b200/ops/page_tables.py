@@ -69,12 +69,11 @@ def step_maps(
             or (width is not None and not 0 < width < 1 << 31)):
         raise KernelError(f"tables {tuple(tables.shape)}, page_size {page_size}, num_tokens {num_tokens} and width {width} do not fit")
     if out is None:
-        device = tables.device
         # the three short ones in one piece of memory
-        q_start, positions, token_entry = torch.empty(entries + 1 + 2 * num_tokens, dtype=torch.int32, device=device).split_with_sizes(
+        q_start, positions, token_entry = tables.new_empty(entries + 1 + 2 * num_tokens).split_with_sizes(
             (entries + 1, num_tokens, num_tokens))
-        out = StepMaps(torch.empty((entries, width or table_width), dtype=torch.int32, device=device), q_start, positions, token_entry,
-                       torch.empty(num_tokens, dtype=torch.int64, device=device))
+        out = StepMaps(tables.new_empty((entries, width or table_width)), q_start, positions, token_entry,
+                       tables.new_empty(num_tokens, dtype=torch.int64))
         pointers = [t.data_ptr() for t in (out.block_table, q_start, positions, token_entry, out.slot_map)]
         if not entries:
             q_start.zero_()

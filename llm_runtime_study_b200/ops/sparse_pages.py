@@ -160,7 +160,7 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
                           "the last ones, of which there is one at least")
     if width > MAX_TABLE_WIDTH:
         raise KernelError(f"block tables of more than {MAX_TABLE_WIDTH} pages are not taken: {width}")
-    chosen = torch.empty((n, kv_heads, budget), dtype=torch.int32, device=q.device)
+    chosen = positions.new_empty((n, kv_heads, budget))
     if n:
         entries = block_table.shape[0]
         tiles, cluster = choose_shape(n, entries, kv_heads, width, d)
