@@ -118,7 +118,7 @@ constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;
 template <int WARPS> __device__ __forceinline__ void sync_group() {
   if (WARPS == 1) __syncwarp(); else __syncthreads();
 }
-constexpr int select_words(int warps) { return 256 + 4 * warps + 3; }
+constexpr int select_words(int warps) { return 256 + 4 * warps + 4; }      // whole 16 bytes
 
 struct Tally {
   uint32_t always, others;      // how many keys are kKeyAlways, how many are candidates
@@ -181,9 +181,11 @@ template <int WARPS> __device__ Border find_border(const uint32_t* keys, int cou
     }
     sync_group<WARPS>();
     if (warp == 0) {       // lane l holds the digits 255 - 8 l down to 248 - 8 l
-      uint32_t mine[8], sum = 0;
+      const uint4 upper = reinterpret_cast<const uint4*>(histogram)[63 - 2 * lane], lower = reinterpret_cast<const uint4*>(histogram)[62 - 2 * lane];
+      const uint32_t mine[8] = {upper.w, upper.z, upper.y, upper.x, lower.w, lower.z, lower.y, lower.x};
+      uint32_t sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine[i] = histogram[255 - 8 * lane - i], sum += mine[i];
+      for (int i = 0; i < 8; ++i) sum += mine[i];
       uint32_t upto = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -348,21 +350,36 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
         for (int i = 0; i < R::per_lane; ++i) low[j][i] = at[part + i * R::lanes], high[j][i] = at[R::chunks + part + i * R::lanes];
       }
     };
-    fetch();           // on their way while the row's numbers are added up
-    double u[R::values], d[R::values];
+    // the row's numbers first: behind the bounds, a full machine's worth of them, they would wait
     const int group = a.q_heads / a.kv_heads;
     const typename L::type* q = reinterpret_cast<const typename L::type*>(static_cast<const T*>(a.q) + (static_cast<size_t>(row) * a.q_heads + head * group) * kDim);
+    constexpr int kFirst = 32 / R::per_lane >= 8 ? 4 : 2;      // heads asked for together
+    typename L::type first[kFirst][R::per_lane];
+#pragma unroll
+    for (int h = 0; h < kFirst; ++h) {
+#pragma unroll
+      for (int i = 0; i < R::per_lane; ++i) first[h][i] = h < group ? q[h * R::chunks + part + i * R::lanes] : typename L::type{};
+    }
+    fetch();
+    double u[R::values], d[R::values];
 #pragma unroll
     for (int i = 0; i < R::values; ++i) u[i] = d[i] = 0;
-#pragma unroll 2
-    for (int h = 0; h < group; ++h) {
+    auto add_head = [&](const typename L::type* row_of_head) {
 #pragma unroll
       for (int i = 0; i < R::per_lane; ++i) {
         float v[L::n];
-        L::unpack(q[h * R::chunks + part + i * R::lanes], v);
+        L::unpack(row_of_head[i], v);
 #pragma unroll
         for (int x = 0; x < L::n; ++x) add_part(v[x], u[i * L::n + x], d[i * L::n + x]);
       }
+    };
+#pragma unroll
+    for (int h = 0; h < kFirst; ++h) add_head(first[h]);
+    for (int h = kFirst; h < group; ++h) {
+      typename L::type more[R::per_lane];
+#pragma unroll
+      for (int i = 0; i < R::per_lane; ++i) more[i] = q[h * R::chunks + part + i * R::lanes];
+      add_head(more);
     }
     // the trip count is the same for all lanes: they exchange sums
     for (int base = from; base < seen; base += stride) {
