@@ -38,6 +38,8 @@ struct Work {
   int row, head, slice, part;
 };
 
+// Rows follow one another head by head: the rows of a prompt that run at once then read the pages of one or two heads, which L2 holds
+// (874 rows: 553 us instead of 587, and as much on pages that are not in L2 yet, where it had been 650).
 __device__ __forceinline__ Work work_of(const AttendArgs& a, int slices) {
   int x = blockIdx.x;
   Work w;
@@ -45,8 +47,8 @@ __device__ __forceinline__ Work work_of(const AttendArgs& a, int slices) {
   x /= a.parts;
   w.slice = x % slices;
   x /= slices;
-  w.head = x % a.kv_heads;
-  w.row = x / a.kv_heads;
+  w.row = x % a.rows;
+  w.head = x / a.rows;
   return w;
 }
 
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(Streams::threads) attend_streams_kernel(const 
 // Eight neighbouring lanes load from two rows, which lie on the same banks of the L1 cache where a row is a multiple of 128 bytes;
 // odd rows then take the blocks of 32 channels of each pair in the other order and exchange the registers afterwards.  (874 prompt
 // rows, 8 kv heads, 2,048 keys each: the data stage of L1 was 91 % busy with values read by columns and both kinds on shared banks, and
-// the kernel took 747 us; 587 now, L1 65 % and L2 56 % busy.)  64 requests of 64 heads over 8, 2,048 keys each: 539 MB in 87 us, 6.2 TB/s.
+// the kernel took 747 us; 553 now.)  64 requests of 64 heads over 8, 2,048 keys each: 539 MB in 87 us, 6.2 TB/s.
 __device__ __forceinline__ uint4 load_row_16(const __nv_bfloat16* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
