@@ -345,13 +345,13 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 && kDim <= 128 ? 16 / WARP
         const int last = here.last - slot;
         if (last < 0) continue;                      // the same for the whole warp
 #pragma unroll
-        for (int i = 0; i < 2; ++i) at[i] = here.page * page_stride + (slot + g + 8 * i) * kDim, is[i] = g + 8 * i <= last;
+        for (int i = 0; i < 2; ++i) at[i] = here.page * page_stride + static_cast<size_t>(slot + g + 8 * i) * kDim, is[i] = g + 8 * i <= last;
       } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int k = tile * 16 + g + 8 * i, place = k / a.page_size, slot = k - place * a.page_size;
           const Place here = place < count ? places[place] : Place{0, -1};
-          at[i] = here.page * page_stride + slot * kDim, is[i] = slot <= here.last;
+          at[i] = here.page * page_stride + static_cast<size_t>(slot) * kDim, is[i] = slot <= here.last;
         }
       }
       uint32_t k0[kRowRegs], k1[kRowRegs], v0[kRowRegs], v1[kRowRegs];

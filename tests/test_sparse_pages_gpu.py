@@ -380,6 +380,30 @@ def test_a_pool_that_needs_more_than_32_bits_of_offset():
     assert torch.equal(out, small.attend(chosen, 0.1))
 
 
+@pytest.mark.parametrize("tail", [16, 8])         # whole tiles of 16 keys, and a page that ends inside one
+def test_a_page_that_needs_more_than_32_bits_of_offset(tail):
+    """One page of more than 2^31 elements: keys that matter in front of that border, at it and behind it.  Those three have the same
+    score, 40 above every other key's, so the row is the mean of their values: 2^24 others weigh 2^24 e^-40 = 7e-11 in all and have
+    values of zero, equal weights are exactly one in bfloat16, so that the rounding of the output (2^-8) is all that is off."""
+
+    d, border = 128, (1 << 31) // 128
+    page = border + tail
+    keys, values = (torch.zeros((1, 1, page, d), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(tail)
+    heavy = torch.randn((3, d), generator=g).to(torch.bfloat16)
+    for at, v in zip((3, border - 1, border + 5), heavy):
+        keys[0, 0, at, 0] = 5.0
+        values[0, 0, at] = v.cuda()
+    q = torch.zeros((1, 2, d), dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 8.0
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")      # noqa: E731
+    rows = dict(token_entry=ints(0), block_table=ints([0]), scale=1.0)
+    for position, seen in ((page - 1, 3), (border + 5, 3), (border + 4, 2), (border - 2, 1)):
+        out = S().paged_attention_chosen(q, keys, values, ints([[0]]), positions=ints(position), **rows)
+        want = heavy[:seen].double().mean(0)
+        assert bool(((out.cpu().double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-6).all()), position
+
+
 # ------------------------------------------------------------------------------------------------------------- together
 def _layer(cache, keys, values, bounds, q, positions, entry, table, q_start, kv_len, budget):
     S().page_bounds(keys, bounds, block_table=table, q_start=q_start, kv_len=kv_len, max_q_len=q.shape[0])
