@@ -307,6 +307,35 @@ def test_attention_over_chosen_pages(dtype, case):
     torch.testing.assert_close(other.float(), out.float(), atol=2e-2 if dtype == torch.bfloat16 else 2e-5, rtol=0)
 
 
+LONG_LISTS = [
+    # length, rows, heads, kv heads, d, page, budget
+    (5000, 1, 4, 2, 64, 1, 4400),
+    (9100, 1, 16, 1, 48, 2, 4500),                # 16 heads in bfloat16: two tiles of heads a CTA
+    (4200 * 16 + 5, 1, 2, 1, 64, 16, 4150),       # whole tiles
+    (1300, 80, 4, 2, 16, 1, 1100),                # bfloat16: rows enough for lists that are not cut, three laps
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", LONG_LISTS)
+def test_lists_longer_than_a_cta_looks_up_at_a_time(dtype, case):
+    """A CTA looks up 512 pages of its part of a list at a time and comes back for more."""
+
+    length, rows, heads, kv_heads, d, page, budget = case
+    parts, _ = S().attention_shape(rows, heads, kv_heads, budget, page, dtype)
+    laps = -(-budget // parts // 512)
+    assert laps >= (3 if rows > 1 and dtype == torch.bfloat16 else 1 if rows > 1 else 2)
+    cache = Cache([length], [rows], heads=heads, kv_heads=kv_heads, d=d, page=page, dtype=dtype, seed=budget)
+    chosen = some_pages(cache, budget)
+    cache.check_attend(chosen)
+    # a list whose later laps alone hold anything
+    late = chosen.clone()
+    late[:, :, : 512 * parts] = -1
+    if laps > 1:
+        assert bool((late >= 0).any(-1).all())
+        cache.check_attend(late)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_large_scores_and_one_heavy_key(dtype):
     cache = Cache([700, 300], [1, 4], heads=8, kv_heads=2, d=64, page=16, dtype=dtype)
