@@ -442,7 +442,8 @@ template <int NT, int WARPS> int launch_mma(const AttendArgs& a, cudaStream_t st
 
 using namespace b200;
 
-// parts: CTAs of a cluster that share out a list; wide: eight warps to a CTA where there is such a kernel (bfloat16).
+// parts: CTAs of a cluster that share out a list; wide: eight warps to a CTA where there is such a kernel (bfloat16, head sizes up to
+// 128, up to eight heads a group).
 extern "C" int b200_attend_chosen(const void* q, const void* keys, const void* values, const int* chosen, const int* positions,
                                   const int* token_entry, const int* block_table, int table_width, void* out, int rows, int entries,
                                   int q_heads, int kv_heads, int page_size, int num_pages, int budget, float scale, int parts, int wide, int dtype,

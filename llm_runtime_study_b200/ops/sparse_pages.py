@@ -171,22 +171,26 @@ def choose_pages(q: torch.Tensor, bounds: torch.Tensor, *, positions: torch.Tens
 
 
 @lru_cache(maxsize=4096)
-def attention_shape(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype) -> tuple[int, bool]:
+def attention_shape(rows: int, heads: int, kv_heads: int, budget: int, page_size: int, dtype: torch.dtype, head_dim: int = 128) -> tuple[int, bool]:
     """(CTAs of a cluster that the list of a row and kv head is cut over: 1, 2, 4 or 8; twice the warps a CTA).  No part is shorter than
     128 keys.  float32: from the list's length alone, so that the order of the sums does not depend on the batch.  bfloat16: as many
-    parts as let two CTAs of eight warps a multiprocessor be there at once; CTAs of four warps where there are more rows than that (32
-    heads over 8 of 128, 2,048 keys a row, parts and "w" for eight warps: 1 request 8: 8.5, 8w: 7.8 us; 8 requests 8: 16.7, 4w: 16.4; 16
-    requests 2: 30.4, 4: 26.8, 1w: 29.0, 2w: 26.6; 32 requests 1: 51.6, 2: 48.5, 1w: 46.1, 2w: 51.1; 40 requests 1: 64, 1w: 72, 2w: 72)."""
+    parts as let two CTAs a multiprocessor be there at once.  A CTA has eight query heads, sixteen of larger groups up to head size 128.
+    CTAs of eight heads up to that size have eight warps while the GPU is not full, others always four (2,048 keys a row, parts and "w" for
+    eight warps; 32 heads over 8 of 128: 1 request 8: 8.5, 8w: 7.8 us; 8 requests 8: 16.7, 4w: 16.4; 16 requests 2: 30.4, 4: 26.8,
+    1w: 29.0, 2w: 26.6; 32 requests 1: 51.6, 2: 48.5, 1w: 46.1, 2w: 51.1; 40 requests 1: 64, 1w: 72, 2w: 72; 64 heads over 4 of 128:
+    8 requests 2: 31.1, 4: 19.8, 8: 15.8; 16 requests 1: 46.0, 2: 32.0, 4: 22.6, 8: 30.6; 32 requests 1: 47.4, 2: 36.5, 4: 43.5; 16 heads
+    over 4 of 256: 16 requests 2: 34.8, 4: 27.8, 8: 33.7)."""
 
     keys, parts = budget * page_size, 1
     if dtype == torch.float32:
         while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128:
             parts *= 2
         return parts, False
-    ctas = rows * kv_heads * -(-(heads // kv_heads) // 8)
+    group = heads // kv_heads
+    ctas = rows * kv_heads * -(-group // (16 if group > 8 and head_dim <= 128 else 8))
     while parts < 8 and 2 * parts <= budget and keys // (2 * parts) >= 128 and 2 * parts * ctas <= 2 * native.sm_count():
         parts *= 2
-    return parts, ctas * parts <= 2 * native.sm_count()
+    return parts, group <= 8 and head_dim <= 128 and ctas * parts <= 2 * native.sm_count()
 
 
 def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, chosen: torch.Tensor, *, positions: torch.Tensor,
@@ -214,6 +218,6 @@ def paged_attention_chosen(q: torch.Tensor, keys: torch.Tensor, values: torch.Te
     if n:
         native.call("b200_attend_chosen", q_at, at, values_at, chosen_at, positions_at, entry_at, table_at, width, out.data_ptr(), n,
                     block_table.shape[0], heads, kv_heads, page_size, pages, budget, float(scale),
-                    *attention_shape(n, heads, kv_heads, budget, page_size, keys.dtype), native.DTYPE_TAG[keys.dtype], stream_ptr(),
+                    *attention_shape(n, heads, kv_heads, budget, page_size, keys.dtype, d), native.DTYPE_TAG[keys.dtype], stream_ptr(),
                     library=library)
     return out

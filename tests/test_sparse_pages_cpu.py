@@ -232,3 +232,15 @@ def test_shapes_of_the_launches():
     assert [attend(n, 32, 8, 128, 16, bf16) for n in (1, 8, 16, 24, 40)] == [(8, True), (4, True), (2, True), (1, True), (1, False)]
     assert attend(1, 32, 8, 4, 16, bf16) == (1, True) and attend(1, 8, 8, 1, 4096, bf16) == (1, True)      # one page is one part
     assert attend(1, 32, 8, 128, 16, f32) == attend(4000, 32, 8, 128, 16, f32) == (8, False)               # the list alone decides
+
+
+def test_shapes_count_the_ctas_that_are_launched():
+    """Groups of more than eight heads: sixteen a CTA up to head size 128, and no CTAs of eight warps; none at larger head sizes."""
+
+    attend = lambda n, heads, kv_heads, d: sparse_pages.attention_shape.__wrapped__(n, heads, kv_heads, 128, 16, torch.bfloat16, d)      # noqa: E731
+    assert [attend(n, 64, 4, 128) for n in (1, 8, 12, 16, 32, 48)] == [(p, False) for p in (8, 8, 4, 4, 2, 1)]
+    assert [attend(n, 96, 8, 64) for n in (4, 8, 16, 24)] == [(p, False) for p in (8, 4, 2, 1)]
+    assert [attend(n, 96, 4, 128) for n in (4, 16, 32)] == [(p, False) for p in (8, 2, 1)]       # 24 heads a group: two CTAs
+    assert [attend(n, 16, 4, 256) for n in (8, 16, 32)] == [(p, False) for p in (8, 4, 2)]
+    assert [attend(n, 64, 4, 256) for n in (8, 16, 32)] == [(p, False) for p in (4, 2, 1)]       # 16 heads a group: two CTAs there
+    assert attend(8, 32, 8, 128) == (4, True)
