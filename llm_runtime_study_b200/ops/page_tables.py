@@ -75,8 +75,6 @@ def step_maps(
         out = StepMaps(tables.new_empty((entries, width or table_width)), q_start, positions, token_entry,
                        tables.new_empty(num_tokens, dtype=torch.int64))
         pointers = [t.data_ptr() for t in (out.block_table, q_start, positions, token_entry, out.slot_map)]
-        if not entries:
-            q_start.zero_()
     else:
         if width is not None and out.block_table.shape[-1] != width:
             raise KernelError(f"out.block_table has {out.block_table.shape[-1]} columns, not {width}")
@@ -91,7 +89,10 @@ def step_maps(
             pointers.append(pointer(t, f"out.{name}", here, dtype, dims=dims, align=dtype.itemsize))
             if t.shape[0] < least:
                 raise KernelError(f"out.{name} has room for {t.shape[0]}, {least} are needed")
-    if entries:
+    if not entries:
+        if out.q_start is not None:
+            out.q_start[:1].zero_()       # the sum over no entries
+    else:
         native.call("b200_step_maps", at, table_rows, table_width, slots_at, kv_len_at, counts_at, pointers[0], out.block_table.shape[1],
                     *pointers[1:], entries, int(page_size), int(num_tokens), native.stream_ptr())
     return out

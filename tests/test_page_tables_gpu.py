@@ -113,3 +113,14 @@ def test_no_entries():
     got = P().step_maps(ints([[1]]), slots=ints([]), kv_len=ints([]), counts=ints([]), page_size=4, num_tokens=0)
     assert got.block_table.shape == (0, 1) and got.q_start.tolist() == [0] and got.positions.numel() == 0
     P().page_table_set(ints([[1]]), rows=ints([]), columns=ints([]), pages=ints([]))
+
+
+def test_no_entries_into_tensors_that_are_there():
+    def full(*shape, dtype=torch.int32):
+        return torch.full(shape, 77, dtype=dtype, device="cuda")
+
+    out = P().StepMaps(full(3, 4), full(4), full(5), full(5), full(5, dtype=torch.int64))
+    assert P().step_maps(ints([[1]]), slots=ints([]), kv_len=ints([]), counts=ints([]), page_size=4, num_tokens=0, out=out) is out
+    assert out.q_start.tolist() == [0, 77, 77, 77]
+    for t in (out.block_table, out.positions, out.token_entry, out.slot_map):
+        assert bool((t == 77).all())
