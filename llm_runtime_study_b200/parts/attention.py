@@ -170,8 +170,10 @@ class GroupedQueryAttention(Mixer):
         if q.dtype == torch.bfloat16 and not ctx.all_decode and ctx.max_kv_len <= self.attention_pages * cache.page_size:
             return ctx.attention(q, cache, scale=self.scale)      # portions of prompts that no row would choose from
         rows = {"positions": ctx.positions, "token_entry": ctx.token_entry, "block_table": table}
-        chosen = sparse_pages.choose_pages(q, bounds, page_size=cache.page_size, budget=self.attention_pages, first=FIRST_PAGES,
-                                           last=LAST_PAGES, **rows)
+        # a list has as many places as the budget has pages: no more than the longest sequence has
+        longest = ctx.manager.groups[cache.group].pages_for(ctx.manager.max_seq_len)
+        budget = min(self.attention_pages, max(longest, FIRST_PAGES + LAST_PAGES))
+        chosen = sparse_pages.choose_pages(q, bounds, page_size=cache.page_size, budget=budget, first=FIRST_PAGES, last=LAST_PAGES, **rows)
         return sparse_pages.paged_attention_chosen(q, cache.keys, cache.values, chosen, scale=self.scale, **rows)
 
 

@@ -87,6 +87,20 @@ def test_a_budget_of_all_pages_is_attention_over_all_tokens(tmp_path, dtype):
         assert float((a - b).abs().max()) < (1e-4 if dtype == "float32" else 6e-2) * scale
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_budget_beyond_any_sequence_is_one_of_all_pages(tmp_path, dtype):
+    """Lists are no longer than the longest sequence's pages, whatever number was given."""
+
+    from llm_runtime_study_b200.engine.runtime import load
+
+    loaded, raw, weights, page = _load(tmp_path, "B", dtype, 10 ** 9)
+    fits = load(tmp_path / "m", device="cuda:0", dtype=dtype, attention_pages=-(-256 // page))
+    tokens = helpers.random_tokens(random.Random(5), raw["vocab_size"], 150)
+    for cuts in ([150], [100, 47, 1, 1, 1]):
+        a, b = (_step_all(x, page, tokens, cuts)[0] for x in (loaded, fits))
+        assert torch.equal(a, b)
+
+
 def test_portions_batches_and_new_pages_do_not_change_a_bit(tmp_path):
     """float32: a sequence's logits however its prompt is cut, beside other requests, and after a roll-back."""
 

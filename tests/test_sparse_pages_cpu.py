@@ -244,3 +244,23 @@ def test_shapes_count_the_ctas_that_are_launched():
     assert [attend(n, 16, 4, 256) for n in (8, 16, 32)] == [(p, False) for p in (8, 4, 2)]
     assert [attend(n, 64, 4, 256) for n in (8, 16, 32)] == [(p, False) for p in (4, 2, 1)]       # 16 heads a group: two CTAs there
     assert attend(8, 32, 8, 128) == (4, True)
+
+
+@pytest.mark.parametrize("max_seq_len,pages,want", [(400, 10, 10), (400, 10 ** 9, 25), (400, 25, 25), (20, 10 ** 9, 3), (20, 3, 3)])
+def test_a_layer_asks_for_no_more_pages_than_a_sequence_has(monkeypatch, max_seq_len, pages, want):
+    from types import SimpleNamespace
+
+    from llm_runtime_study_b200.parts.attention import GroupedQueryAttention
+
+    asked = []
+    monkeypatch.setattr(sparse_pages, "page_bounds", lambda *a, **k: None)
+    monkeypatch.setattr(sparse_pages, "choose_pages", lambda *a, budget, **k: asked.append(budget))
+    monkeypatch.setattr(sparse_pages, "paged_attention_chosen", lambda q, *a, **k: q)
+    pool = SimpleNamespace(pages_for=lambda n: -(-n // 16))
+    ctx = SimpleNamespace(manager=SimpleNamespace(groups=[pool], max_seq_len=max_seq_len), q_start=None, kv_len=None, max_q_len=1,
+                          all_decode=True, positions=None, token_entry=None)
+    cache = SimpleNamespace(group=0, page_size=16, keys=None, values=None)
+    part = SimpleNamespace(shares_kv=False, attention_pages=pages, scale=1.0)
+    q = torch.zeros(1, 4, 64)
+    assert GroupedQueryAttention._attend_chosen(part, q, ctx, cache, None, None) is q
+    assert asked == [want]
