@@ -103,8 +103,12 @@ def resolve_attention_pages(requested: int | None) -> int | None:
 def _check_attention_pages(loaded: LoadedModel) -> LoadedModel:
     if loaded.runtime.attention_pages is not None:
         groups = loaded.model.cache_layout().groups
-        if not any(name == "bounds" for group in groups for name, _ in group.requirement.page_tensors):
+        bounds = [shape for group in groups for name, shape in group.requirement.page_tensors if name == "bounds"]
+        if not bounds:
             raise EngineError("attention_pages was given, but no layer of this model chooses pages (kind gqa_attention without a window)")
+        for shape in bounds:
+            if not sparse_pages.supported(shape[-1]):
+                raise EngineError(f"attention_pages takes head sizes that are multiples of 16 up to 256, not {shape[-1]}")
     return loaded
 
 

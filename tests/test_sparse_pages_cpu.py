@@ -264,3 +264,22 @@ def test_a_layer_asks_for_no_more_pages_than_a_sequence_has(monkeypatch, max_seq
     q = torch.zeros(1, 4, 64)
     assert GroupedQueryAttention._attend_chosen(part, q, ctx, cache, None, None) is q
     assert asked == [want]
+
+
+@pytest.mark.parametrize("head_dim,taken", [(16, True), (128, True), (256, True), (8, False), (24, False), (272, False)])
+def test_head_sizes_are_refused_when_a_model_is_loaded(head_dim, taken):
+    from types import SimpleNamespace
+
+    from llm_runtime_study_b200.cache.manager import CacheLayout
+    from llm_runtime_study_b200.engine.runtime import _check_attention_pages
+    from llm_runtime_study_b200.errors import EngineError
+    from llm_runtime_study_b200.parts.base import PagedKV
+
+    needs = [PagedKV(2, 64, window=9), PagedKV(2, head_dim, page_tensors=(("bounds", (2, 2, head_dim)),))]
+    model = SimpleNamespace(cache_layout=lambda: CacheLayout.from_requirements(needs))
+    loaded = SimpleNamespace(model=model, runtime=SimpleNamespace(attention_pages=8))
+    if taken:
+        assert _check_attention_pages(loaded) is loaded
+    else:
+        with pytest.raises(EngineError, match="head sizes"):
+            _check_attention_pages(loaded)
