@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t score_key(double score) {
 // Pages that a row sees: 0 for a row that stands nowhere (an entry that is none, a negative position).
 __device__ __forceinline__ int visible_pages(const ChooseArgs& a, int position, int entry) {
   if (position < 0 || entry < 0 || entry >= a.entries) return 0;
-  return min(position / a.page_size + 1, a.table_width);
+  return min(position / a.page_size, a.table_width - 1) + 1;
 }
 
 constexpr int kChooseThreads = 256, kChooseWarps = kChooseThreads / 32;

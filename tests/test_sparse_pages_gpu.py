@@ -274,6 +274,20 @@ def test_rows_that_stand_nowhere_and_pages_that_are_not_held(dtype):
         assert float(out[[1, 3, 4]].abs().max()) == 0.0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_last_position_there_is(dtype):
+    """Pages of one token: a page's number and the count of pages up to it are 32-bit numbers, and the count must not wrap."""
+
+    cache = Cache([70, 70, 70, 70], [1, 1, 1, 1], heads=4, kv_heads=2, d=64, page=1, dtype=dtype)
+    cache.positions[1] = 2 ** 31 - 1
+    cache.positions[2] = 2 ** 31 - 2
+    for budget in (5, 100):
+        got = cache.choose(budget, 1, 2)
+        assert torch.equal(got.cpu(), cache.plain_choose(budget, 1, 2))
+        assert bool((got[1] >= 0).any())
+        cache.check_attend(got)
+
+
 # ------------------------------------------------------------------------------------------------------------ attention
 ATTENTION = [
     # lengths, counts, heads, kv heads, d, page, budget
