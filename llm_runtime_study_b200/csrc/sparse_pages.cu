@@ -551,6 +551,10 @@ inline bool fits(const ChooseArgs& a) {
          (a.cluster == 1 || a.cluster == 2 || a.cluster == 4 || a.cluster == 8);
 }
 
+// Of this build alone: a static of a template that several loaded libraries share by name would be one for all of them, and the shared
+// memory of another head size's kernel would go without its limit being raised.
+namespace {
+
 template <typename T> int launch_choose(const ChooseArgs& a, cudaStream_t stream) {
   static DeviceOnce once;
   const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * a.cluster, bytes = static_cast<long long>(a.table_width) * 4;
@@ -570,6 +574,7 @@ template <typename T> int launch_choose_tiles(const ChooseArgs& a, cudaStream_t 
   return launch_status();
 }
 
+}  // namespace
 }  // namespace b200
 
 using namespace b200;

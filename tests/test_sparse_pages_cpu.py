@@ -283,3 +283,24 @@ def test_head_sizes_are_refused_when_a_model_is_loaded(head_dim, taken):
     else:
         with pytest.raises(EngineError, match="head sizes"):
             _check_attention_pages(loaded)
+
+
+def test_no_static_is_shared_by_libraries_that_configure_kernels_of_their_own():
+    """What a library remembers of its kernels' configuration must not be one object for all builds of the same source (exported names of
+    the libraries that are built)."""
+
+    import collections
+    import pathlib
+    import shutil
+    import subprocess
+
+    from llm_runtime_study_b200.csrc import build
+
+    built = sorted(pathlib.Path(build.CSRC_DIR, "_build").glob("lib*.so"))
+    if not built or shutil.which("nm") is None:
+        pytest.skip("no libraries are built here")
+    shared = collections.Counter()
+    for path in built:
+        names = subprocess.run(["nm", "-D", "--defined-only", str(path)], capture_output=True, text=True, check=True).stdout.splitlines()
+        shared.update(name.split()[-1] for name in names if name.split()[-2] == "u")
+    assert [name for name, n in shared.items() if n > 1 and name.endswith("4once")] == []

@@ -197,6 +197,25 @@ def test_many_pages(rows):
         assert torch.equal(got[i, 0].long(), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_head_sizes_one_after_the_other_in_one_process(dtype):
+    """Every head size is a library of its own, and each has to raise its kernels' limit of shared memory: the scores of 13,000 pages
+    are more than a kernel gets unasked."""
+
+    for d in (64, 128, 32, 256, 16):
+        for length, rows in ((13000, 8), (13000, 1)):
+            cache = Cache([length], [rows], heads=2, kv_heads=1, d=d, page=1, dtype=dtype, seed=d)
+            got = cache.choose(40, 1, 2).cpu()
+            x = cache.q.double()
+            b = cache.bounds[cache.table[0, :length].long(), 0].double()
+            score = (x.clamp(min=0).sum(1) @ b[:, 1].T + x.clamp(max=0).sum(1) @ b[:, 0].T).float()
+            for i in range(rows):
+                seen = int(cache.positions[i]) + 1
+                order = score[i, 1 : seen - 2].argsort(descending=True, stable=True)[:37] + 1
+                want = torch.cat((torch.tensor([0]), order.sort().values, torch.arange(seen - 2, seen)))
+                assert torch.equal(got[i, 0].long(), want), (d, length)
+
+
 @pytest.mark.parametrize("rows", [1, 12])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_equal_scores_go_to_the_lower_page(dtype, rows):
