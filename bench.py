@@ -144,7 +144,7 @@ def run_ours(args) -> dict:
         cfg, seed=0, device="cuda:0", dtype="bfloat16", max_seq_len=cfg["max_position_embeddings"],
         max_batch_size=max_batch, page_size=PAGE_SIZE,
         max_cache_tokens=max_batch * (context + args.steps + max_batch + max(args.warmup, 3) + 2 * PAGE_SIZE),
-        max_tokens_per_step=PREFILL_TOKENS, use_cuda_graph=True)
+        max_tokens_per_step=PREFILL_TOKENS, use_cuda_graph=True, attention_pages=args.attention_pages or None)
     runner, manager = engine.runner, engine.cache_manager
     sampler = engine._sampler
     greedy = SlotRecord(position=0)          # temperature 0: the largest logit
@@ -208,10 +208,31 @@ def run_ours(args) -> dict:
             manager.release(request)
         return ms, launches, info
 
-    if args.only == "decode":   # profiling aid: nothing but the decode steps of one batch size
+    def prompt_point():
+        """Milliseconds of a prompt of the context's length in portions, and of its last portion."""
+
+        request, tokens = manager.admit(), ids(context)
+        events = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        torch.cuda.synchronize()
+        events[0].record()
+        for at in range(0, context, PREFILL_TOKENS):
+            part = tokens[at : at + PREFILL_TOKENS]
+            last = at + len(part) == context
+            if last:
+                events[1].record()
+            runner.step_sampled([StepEntry(request, part, [len(part) - 1] if last else [], greedy if last else None)], sampler)
+        events[2].record()
+        torch.cuda.synchronize()
+        manager.release(request)
+        return events[0].elapsed_time(events[2]), events[1].elapsed_time(events[2])
+
+    if args.only == "decode":   # profiling aid: nothing but prompts and decode steps of one batch size and context length
+        prompt_point()
+        prompts = [prompt_point() for _ in range(3)]
         ms, launches, _ = decode_point(args.batch, args.steps, args.warmup)
-        return {"only": "decode", "layers": layers, "batch": args.batch, "context": context, "ms_per_step": round(ms, 4),
-                "gpu_launches": launches}
+        return {"only": "decode", "layers": layers, "batch": args.batch, "context": context, "attention_pages": args.attention_pages or None,
+                "ms_per_step": round(ms, 4), "gpu_launches": launches, "prompt_ms": round(statistics.median(p for p, _ in prompts), 1),
+                "last_portion_ms": round(statistics.median(p for _, p in prompts), 2)}
     ms_b8, launches, clocks = decode_point(args.batch, args.steps, args.warmup, sample_clocks=True)
     ms_b1, _, _ = decode_point(1, args.steps, args.warmup)
     ms_b64, _, _ = decode_point(64, args.steps, args.warmup)
@@ -219,8 +240,9 @@ def run_ours(args) -> dict:
     # ------------------------------------- end to end through the scheduler
     def end_to_end(batch):
         """Tokens per second by the wall clock through the scheduler that ``Engine.generate`` drives:
-        requests in as host token ids, events with token ids out.  Every step copies its slots and block
-        tables from pinned host memory to the device and the drawn ids back into pinned host memory."""
+        requests in as host token ids, events with token ids out.  Every step copies its slots, and the places of
+        the block tables that changed (a page that a request has taken), from pinned host memory to the device and
+        the drawn ids back into pinned host memory."""
 
         engine.max_batch_size = batch
         scheduler = engine.create_scheduler()
@@ -233,6 +255,13 @@ def run_ours(args) -> dict:
         graph = runner._graphs.graph_for(batch) if runner._graphs else None
         if graph is not None:
             graph.always_send = True          # copy the step's inputs every step, changed or not
+        uploads, upload = [], runner._buffers.upload
+
+        def counted(packed):
+            uploads.append(packed.nbytes)
+            return upload(packed)
+
+        runner._buffers.upload = counted
         gc.collect()                          # a collection of the host's garbage inside a 60 ms region is milliseconds of noise
         gc.disable()
         try:
@@ -245,9 +274,10 @@ def run_ours(args) -> dict:
             seconds = time.perf_counter() - t0
         finally:
             gc.enable()
+            del runner._buffers.upload
         scheduler.abort_all()
         torch.cuda.synchronize()
-        return produced / seconds, (graph.sent * 4 if graph else 0), batch * 4
+        return produced / seconds, (graph.sent * 4 if graph else 0) + round(sum(uploads) / args.steps), batch * 4
 
     e2e_b8, h2d, d2h = end_to_end(args.batch)
     e2e_b1, _, _ = end_to_end(1)
@@ -1784,6 +1814,8 @@ def main() -> int:
     parser.add_argument("--impl", choices=("ours", "reference"), default="ours")
     parser.add_argument("--batch", type=int, default=8)
     parser.add_argument("--context", type=int, default=0, help="with --only decode: cached tokens per request (default 2048)")
+    parser.add_argument("--attention-pages", type=int, default=0,
+                        help="with --only decode: every token reads at most so many pages of keys and values (default: all)")
     parser.add_argument("--layers", type=int, default=0, help="fewer layers than the configuration has (named in config)")
     parser.add_argument("--workload", choices=("default", "staggered14b", "decode32b", "sorulix", "ropulix", "mabedra", "tafisun", "fumolorn", "refolix"), default="default",
                         help="default: Qwen3-8B decode/prefill; staggered14b, decode32b: the larger configurations (either --impl); "
@@ -1798,6 +1830,8 @@ def main() -> int:
                         help="run only the decode steps or only the prefill (for profiler captures of a small case); "
                              "with --workload sorulix: only the kernels alone, or only the whole models")
     args = parser.parse_args()
+    if args.attention_pages and args.only != "decode":
+        parser.error("--attention-pages goes with --only decode")
     if args.gpus != 1:
         print(f"bench.py measures one GPU: --gpus {args.gpus} is not supported by this engine (single-GPU tier)")
         return 2
