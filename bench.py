@@ -257,9 +257,9 @@ def run_ours(args) -> dict:
             graph.always_send = True          # copy the step's inputs every step, changed or not
         uploads, upload = [], runner._buffers.upload
 
-        def counted(packed):
-            uploads.append(packed.nbytes)
-            return upload(packed)
+        def counted(pieces, offsets):
+            uploads.append(4 * offsets[-1])
+            return upload(pieces, offsets)
 
         runner._buffers.upload = counted
         gc.collect()                          # a collection of the host's garbage inside a 60 ms region is milliseconds of noise

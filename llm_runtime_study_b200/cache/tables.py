@@ -31,6 +31,18 @@ class DeviceTables:
         self.tensors = [torch.full((slots + 1, width), -1, dtype=torch.int32, device=device) for width in widths]
         self._known: dict[int, _Known] = {}
 
+    def current(self, requests: Sequence) -> bool:
+        """Whether the device's rows of these requests are the host's already (what most decode steps find)."""
+
+        for request in requests:
+            known = self._known.get(request.slot)
+            if known is None or known.request != request.id:
+                return False
+            for table, columns, back in zip(request.tables, known.columns, known.given_back):
+                if columns != len(table) or (back < columns and table[back] < 0):
+                    return False
+        return True
+
     def changes(self, requests: Sequence) -> list[np.ndarray]:
         """The cells that differ from what the device holds: for every group their rows, columns and pages (int32)."""
 

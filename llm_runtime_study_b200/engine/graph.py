@@ -110,10 +110,8 @@ class DecodeGraph:
 
         b = self.batch
         runner, manager = self.runner, self.runner.manager
-        if manager.tables is not None:
-            changes = manager.tables.changes(requests)
-            if any(cells.size for cells in changes):
-                runner.set_tables(requests, runner._send(changes))
+        if manager.tables is not None and not manager.tables.current(requests):
+            runner.set_tables(requests, runner._send(manager.tables.changes(requests)))
         sent = np.zeros(self.sent, dtype=np.int32)
         sent[:b] = manager.padding_slot
         sent[: len(requests)] = [r.slot for r in requests]

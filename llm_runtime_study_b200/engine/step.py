@@ -76,7 +76,7 @@ class StepContext:
         self.kv_len: torch.Tensor = None         # [R] int32 length of each request after this step
         self.slots: torch.Tensor = None          # [R] int32 request slot of each entry
         self.logit_rows: torch.Tensor = None     # [M] int32 rows whose logits are wanted
-        self.counts: torch.Tensor = None         # [R] int32 new tokens of each entry
+        self.counts: torch.Tensor | None = None  # [R] int32 new tokens of each entry, where a kernel needed them
         self.tables: list[torch.Tensor] = []     # per page group: [R, width] int32
         self._slot_maps: dict[int, torch.Tensor] = {}
         # host-side copies, for choosing kernels and grids
@@ -105,6 +105,8 @@ class StepContext:
             made = torch.empty(self.num_tokens, dtype=torch.int64, device=tables.device)
             out = page_tables.StepMaps(torch.empty_like(tables), slot_map=made)
             rows = torch.arange(tables.shape[0], dtype=torch.int32, device=tables.device)
+            if self.counts is None:
+                self.counts = self.q_start[1:] - self.q_start[:-1]
             page_tables.step_maps(tables, slots=rows, kv_len=self.kv_len, counts=self.counts, page_size=self.manager.groups[group].page_size,
                                   num_tokens=self.num_tokens, out=out)
             if not self.captured:       # a captured step's map belongs to the graph: every replay makes it anew
@@ -125,6 +127,7 @@ class _MetaBuffers:
         self.device = device
         self.capacity = 0
         self.host: list[torch.Tensor] = []
+        self.views: list[np.ndarray] = []
         self.events: list[torch.cuda.Event | None] = []
         self.dev: torch.Tensor | None = None
         self.turn = 0
@@ -138,20 +141,24 @@ class _MetaBuffers:
         self.capacity = capacity
         pin = self.device.type == "cuda"
         self.host = [torch.empty(capacity, dtype=torch.int32, pin_memory=pin) for _ in range(self.RING)]
+        self.views = [host.numpy() for host in self.host]
         self.events = [None] * self.RING
         self.dev = torch.empty(capacity, dtype=torch.int32, device=self.device)
 
-    def upload(self, packed: np.ndarray) -> torch.Tensor:
-        n = packed.shape[0]
+    def upload(self, pieces: Sequence[np.ndarray], offsets: Sequence[int]) -> torch.Tensor:
+        """The int32 pieces, each from its offset on, in one copy; ``offsets`` ends with the number of words."""
+
+        n = offsets[-1]
         self._reserve(max(n, 1))
         self.turn = (self.turn + 1) % self.RING
         event = self.events[self.turn]
         if event is not None:
             event.synchronize()
-        host = self.host[self.turn]
-        host[:n].numpy()[:] = packed
+        view = self.views[self.turn]
+        for piece, at in zip(pieces, offsets):
+            view[at : at + piece.size] = piece if piece.ndim == 1 else piece.reshape(-1)
         dev = self.dev[:n]
-        dev.copy_(host[:n], non_blocking=True)
+        dev.copy_(self.host[self.turn][:n], non_blocking=True)
         if self.device.type == "cuda":
             event = event or torch.cuda.Event()
             event.record()
@@ -248,15 +255,11 @@ class StepRunner:
     def _send(self, pieces: Sequence[np.ndarray]) -> list[torch.Tensor]:
         """The int32 pieces on the device, in one copy; each starts on a 16-byte boundary."""
 
-        sizes = []      # of a piece, and of the words up to the next one
+        offsets = [0]
         for piece in pieces:
-            sizes += [piece.size, -piece.size % 4]
-        packed = np.zeros(sum(sizes), dtype=np.int32)
-        off = 0
-        for piece, size in zip(pieces, sizes[::2]):
-            packed[off : off + size] = piece.reshape(-1)
-            off += size + -size % 4
-        parts = self._buffers.upload(packed).split_with_sizes(sizes)[::2]
+            offsets.append(offsets[-1] + piece.size + -piece.size % 4)
+        dev = self._buffers.upload(pieces, offsets)
+        parts = [dev[at : at + piece.size] for piece, at in zip(pieces, offsets)]
         return [part if piece.ndim == 1 else part.view(piece.shape) for part, piece in zip(parts, pieces)]
 
     def _tables_on_device(self, requests: Sequence[RequestCache]) -> bool:
@@ -313,19 +316,20 @@ class StepRunner:
                 e.sample = replace(e.sample, position=length)
         for i, e in enumerate(sampled):
             staged[i] = manager.slots.note(e.request.slot, e.sample)
-        pieces = [token_ids, np.asarray(kv_lens, dtype=np.int32), np.asarray(q_lens, dtype=np.int32), slots, logit_rows, row_slots, staged]
+        pieces = [token_ids, np.asarray(kv_lens, dtype=np.int32), slots, logit_rows, row_slots, staged]
 
         ctx = StepContext(self.runtime, manager)
         ctx.num_tokens, ctx.num_entries, ctx.num_logit_rows = num_tokens, num_entries, int(logit_rows.shape[0])
         if self._tables_on_device(requests):
             # the requests' tables are on the device already: what changed of them goes there, the rest is made there
-            sent = self._send([*pieces, *manager.tables.changes(requests)])
-            self.set_tables(requests, sent[len(pieces) :])
+            sent = self._send([*pieces, np.asarray(q_lens, dtype=np.int32), *manager.tables.changes(requests)])
+            ctx.counts = sent[len(pieces)]
+            self.set_tables(requests, sent[len(pieces) + 1 :])
             tables = self._empty_tables(requests, table_width)
             sizes = (num_entries + 1, -(num_entries + 1) % 4, num_tokens, -num_tokens % 4, num_tokens)     # on 16-byte boundaries, too
             ints = torch.empty(sum(sizes), dtype=torch.int32, device=self.runtime.device).split_with_sizes(sizes)[::2]
             for g, table in enumerate(tables):
-                page_tables.step_maps(manager.tables.tensors[g], slots=sent[3], kv_len=sent[1], counts=sent[2],
+                page_tables.step_maps(manager.tables.tensors[g], slots=sent[2], kv_len=sent[1], counts=ctx.counts,
                                       page_size=manager.groups[g].page_size, num_tokens=num_tokens,
                                       out=page_tables.StepMaps(table, *(ints if g == 0 else ())))
             ctx.q_start, ctx.positions, ctx.token_entry = ints
@@ -335,7 +339,7 @@ class StepRunner:
             sent = self._send([*pieces, q_start, positions, token_entry, *self._host_tables(requests, table_width)])
             ctx.q_start, ctx.positions, ctx.token_entry = sent[len(pieces) : len(pieces) + 3]
             tables = sent[len(pieces) + 3 :]
-        ctx.token_ids, ctx.kv_len, ctx.counts, ctx.slots, ctx.logit_rows, ctx.row_slots, ctx.staged_records = sent[: len(pieces)]
+        ctx.token_ids, ctx.kv_len, ctx.slots, ctx.logit_rows, ctx.row_slots, ctx.staged_records = sent[: len(pieces)]
         ctx.tables = list(tables)
         ctx.q_lens, ctx.kv_lens = q_lens, kv_lens
         ctx.entry_slots = [r.slot for r in requests]

@@ -304,3 +304,44 @@ def test_no_static_is_shared_by_libraries_that_configure_kernels_of_their_own():
         names = subprocess.run(["nm", "-D", "--defined-only", str(path)], capture_output=True, text=True, check=True).stdout.splitlines()
         shared.update(name.split()[-1] for name in names if name.split()[-2] == "u")
     assert [name for name, n in shared.items() if n > 1 and name.endswith("4once")] == []
+
+
+def test_tables_are_current_when_nothing_of_them_changed():
+    """``DeviceTables.current`` says of random histories (pages taken, given back by a window, slots reused) what ``changes`` says."""
+
+    import random
+    from types import SimpleNamespace
+
+    from llm_runtime_study_b200.cache.tables import DeviceTables
+
+    rng = random.Random(3)
+    tables = DeviceTables(4, [20, 20], torch.device("cpu"))
+    copies = [t.tolist() for t in tables.tensors]
+    live, seen = {}, {True: 0, False: 0}
+    for step in range(3000):
+        slot = rng.randrange(4)
+        if slot not in live or rng.random() < 0.1:
+            live[slot] = SimpleNamespace(slot=slot, id=step, tables=[[], []])
+        request = live[slot]
+        for table in request.tables:
+            if len(table) < 20 and rng.random() < 0.2:
+                table.extend(rng.randrange(100) for _ in range(rng.randint(1, 3)) if len(table) < 18)
+            back = sum(page < 0 for page in table)
+            if back < len(table) and rng.random() < 0.1:
+                table[back] = -1
+        batch = rng.sample(sorted(live), rng.randint(1, len(live)))
+        batch = [live[s] for s in batch]
+        changes = tables.changes(batch)
+        current = tables.current(batch)
+        assert current or any(cells.size for cells in changes) or any(not any(r.tables) for r in batch)
+        assert not current or not any(cells.size for cells in changes)
+        seen[current] += 1
+        for g, copy in enumerate(copies):
+            for r, c, page in zip(*(cells.tolist() for cells in changes[3 * g : 3 * g + 3])):
+                copy[r][c] = page
+        tables.sent(batch)
+        assert tables.current(batch) and not any(cells.size for cells in tables.changes(batch))
+        for request in batch:
+            for copy, table in zip(copies, request.tables):
+                assert copy[request.slot][: len(table)] == table
+    assert min(seen.values()) > 100
