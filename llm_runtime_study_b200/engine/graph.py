@@ -150,14 +150,13 @@ class DecodeGraph:
         records = manager.slots.records
         saved = records.clone()
         saved_states = {layer: state.clone() for layer, state in manager.state_arrays.items()}
-        stream = torch.cuda.Stream(device=self.runner.runtime.device)
-        stream.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(stream), torch.inference_mode():
+        # On the stream of the replays: with this run on one of its own, replays took 2 % longer until a step was launched eagerly (Qwen3-8B
+        # shape, batch 1, the second graph captured: 3.18 ms a step instead of 3.11).
+        with torch.inference_mode():
             self._launches(sampler, ids)
             records.copy_(saved)
             for layer, state in saved_states.items():
                 manager.state_arrays[layer].copy_(state)
-        torch.cuda.current_stream().wait_stream(stream)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         before = native.launch_count()
