@@ -76,7 +76,7 @@ def step_maps(
                        tables.new_empty(num_tokens, dtype=torch.int64))
         pointers = [t.data_ptr() for t in (out.block_table, q_start, positions, token_entry, out.slot_map)]
     else:
-        if width is not None and out.block_table.shape[-1] != width:
+        if width is not None and isinstance(out.block_table, torch.Tensor) and out.block_table.shape[-1] != width:
             raise KernelError(f"out.block_table has {out.block_table.shape[-1]} columns, not {width}")
         pointers = []
         for name, dtype, dims, least in (("block_table", torch.int32, 2, entries), ("q_start", torch.int32, 1, entries + 1),

@@ -345,3 +345,19 @@ def test_tables_are_current_when_nothing_of_them_changed():
             for copy, table in zip(copies, request.tables):
                 assert copy[request.slot][: len(table)] == table
     assert min(seen.values()) > 100
+
+
+@pytest.mark.parametrize("width", [None, 4])
+def test_a_block_table_that_is_none_is_refused(host, monkeypatch, width):
+    real = page_tables.pointer
+
+    def pointer(t, name, *args, **kwargs):
+        if not isinstance(t, torch.Tensor):
+            raise KernelError(name)
+        return real(t, name, *args, **kwargs)
+
+    monkeypatch.setattr(page_tables, "pointer", pointer)
+    with pytest.raises(KernelError, match="block_table"):
+        page_tables.step_maps(ints(3, 4), slots=ints(2), kv_len=ints(2), counts=ints(2), page_size=8, num_tokens=4, width=width,
+                              out=page_tables.StepMaps(None))
+    assert host == []
