@@ -65,7 +65,8 @@ def build_parser() -> argparse.ArgumentParser:
     add("--page-size", type=int, default=16)
     add("--max-tokens-per-step", type=int, default=2048)
     add("--attention-pages", type=int, metavar="N",
-        help="read at most N pages of keys and values for a token, the ones that can matter most to it (default: all)")
+        help="read at most N pages of keys and values for a token, the ones that can matter most to it (default: all); "
+             "decoding at long contexts gets faster, long prompts get slower")
     add("--no-cuda-graph", action="store_true")
     add("--any-storage-dtype", action="store_true",
         help="accept weights stored in another floating type than config.json's torch_dtype")

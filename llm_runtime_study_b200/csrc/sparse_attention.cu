@@ -39,7 +39,7 @@ struct Work {
 };
 
 // Rows follow one another head by head: the rows of a prompt that run at once then read the pages of one or two heads, which L2 holds
-// (874 rows: 553 us instead of 587, and as much on pages that are not in L2 yet, where it had been 650).
+// (874 rows: 555 us instead of 587, and 570 on pages that are not in L2 yet, where it had been 650).
 __device__ __forceinline__ Work work_of(const AttendArgs& a, int slices) {
   int x = blockIdx.x;
   Work w;
@@ -126,8 +126,9 @@ __device__ void join_and_write(const AttendArgs& a, const Work& w, float (*sums)
 // ------------------------------------------------------------------------------------------------- float32, CUDA cores
 // A few lanes hold a key's row (RowLanes), each such team walks keys of its own.  Which keys a team takes, and the order of every
 // sum, depend on the list alone: `parts` is chosen from the list's length, not from the batch.  What bounds it is the latency of the
-// keys in flight (registers: queries, values and two keys a team): 90 rows, 2 kv heads of 64, 384 keys 13 us; one row, 8 of 128, 2,048
-// keys 16 us.
+// keys in flight (240 registers: queries, values and two keys a team; 4 warps of a multiprocessor's 64 for one row): 90 rows, 2 kv heads
+// of 64, 384 keys 13 us; one row, 8 of 128, 2,048 keys 16 us, 21 from HBM; 64 rows of 64 heads over 8, 2,048 keys 666 us (1.6 TB/s); 874
+// rows of 16 heads over 8, 2,048 keys 3.7 ms (all their 10,000 to 16,000 keys by the dense kernel: 4.4).
 struct Streams {
   using R = RowLanes<float>;
   static constexpr int threads = 128;
@@ -237,10 +238,16 @@ __global__ void __launch_bounds__(Streams::threads) attend_streams_kernel(const 
 // (and the weights P^T, which come in the layout of the accumulator) are turned by movmatrix, 8x8 numbers across the warp.  No
 // shared memory and no barrier in the loop.
 //
+// Weights are rounded to bfloat16 where they meet the values (one operand type to a product; a second product for what the rounding
+// leaves would be half as much work again); their sum is taken before, in 32 bits.  The rounding errors, 2^-8 of a weight at most, average
+// out over the keys: the outputs' error against 64 bits is 1.7e-3 to 1.8e-3 of their norm, 1.66e-3 being that of the outputs' own rounding.
+//
 // Eight neighbouring lanes load from two rows, which lie on the same banks of the L1 cache where a row is a multiple of 128 bytes;
 // odd rows then take the blocks of 32 channels of each pair in the other order and exchange the registers afterwards.  (874 prompt
 // rows, 8 kv heads, 2,048 keys each: the data stage of L1 was 91 % busy with values read by columns and both kinds on shared banks, and
-// the kernel took 747 us; 553 now.)  64 requests of 64 heads over 8, 2,048 keys each: 539 MB in 87 us, 6.2 TB/s.
+// the kernel took 747 us; 555 now.)  64 requests of 64 heads over 8, 2,048 keys each: 539 MB in 88 us, 6.1 TB/s.  Rows of a prompt are
+// bound by L1's data stage (66 % busy): every row reads its own 8 MB of pages.  Dense tiles over all keys of the same rows, 6.6 times as
+// many, take 250 us.
 __device__ __forceinline__ uint4 load_row_16(const __nv_bfloat16* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));

@@ -40,7 +40,7 @@ struct BoundsArgs {
 
 // A warp takes (entry, page that this step's tokens fill, kv head) triples.  Pages that are not full keep the bounds they
 // have: a row always reads its last page, so nobody asks for them.  Each key is read once, 16 bytes a lane: 511 pages of 16 keys,
-// 8 heads of 128 in bfloat16, 18.8 MB in 4.8 us (3.9 TB/s, a launch's ramp and one round of loads).
+// 8 heads of 128 in bfloat16, 18.8 MB in 7.7 us (2.4 TB/s; 4.8 us where L2 holds the keys): a launch's ramp and one round of loads.
 template <typename T> __global__ void __launch_bounds__(128) page_bounds_kernel(const __grid_constant__ BoundsArgs a) {
   using L = Vec<T>;
   constexpr int kChunks = RowLanes<T>::chunks;
@@ -307,9 +307,10 @@ __device__ __forceinline__ void store_in_cluster(uint32_t address, uint32_t v) {
 
 // Single tokens: a cluster per (row, kv head), whose warps share out the pages; a team of lanes holds U and D in registers and reads
 // a page's bounds 16 bytes a lane, the next pages' ones before these are summed.  Every score's key goes into the first CTA's shared
-// memory, which then chooses.  Scores are summed in 64 bits and rounded once: the products of bfloat16 numbers are exact there, so
-// neither the order of the sum nor its spread over lanes moves a page across the border.  One request of 2,048 pages 11.8 us (latencies
-// in a row), 32 of up to 2,048 pages, 171 MB, 54 us: issue and latency of the 64-bit sums, 16 warps an SM.
+// memory, which then chooses.  Scores are summed in 64 bits and rounded once to 32.  The products of bfloat16 numbers are exact there,
+// the sums are not once their terms lie further apart than 53 bits: a score next to a midpoint of two 32-bit numbers can come out one
+// step apart from the tile kernel's below, which adds in another order.  One request of 2,048 pages 12.5 us (latencies in a row), 32 of
+// up to 2,048 pages, 171 MB, 53 us: issue and latency of the 64-bit sums at 14 warps an SM, and rows of unequal length.
 template <typename T> __global__ void __launch_bounds__(kChooseThreads, ScoreLanes<T>::values <= 8 ? 2 : 1)
 choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
   using L = Vec<T>;
@@ -438,7 +439,7 @@ choose_pages_kernel(const __grid_constant__ ChooseArgs a) {
 // cores (mma.m8n8k4.f64; d sums and u sums against low and high bounds), so that a bound is read and widened once for eight
 // rows.  A lane's four numbers of the sum over channels may be any: it takes the channels of one 16-byte chunk one after the other.
 // The CTAs of the cluster share out the pages, then the rows: one warp chooses for a row.  Rows of several entries in one tile are
-// scored entry by entry.  874 rows of 640 to 1,024 pages, 8 kv heads of 128: 141 us, the 64-bit tensor pipe 66 % busy (a CTA per row:
+// scored entry by entry.  874 rows of 640 to 1,024 pages, 8 kv heads of 128: 140 us, the 64-bit tensor pipe 66 % busy (a CTA per row:
 // 1,733 us).
 constexpr int kTileRows = 8;
 

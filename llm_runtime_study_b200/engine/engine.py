@@ -69,7 +69,8 @@ class Engine:
         by default: every token attends to all tokens before it; a number of at least 3: in
         layers without a window every token, of prompts too, reads at most so many pages of
         keys and values, the first page, the last two and those that can matter most to it
-        by the bounds of their keys)."""
+        by the bounds of their keys; decoding at long contexts gets faster, prompts longer than
+        that many pages get slower in bfloat16, up to 2.2 times)."""
 
         started = time.perf_counter()
         attention_pages = options.pop("attention_pages", None)

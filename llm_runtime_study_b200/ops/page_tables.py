@@ -54,7 +54,7 @@ def step_maps(
     """The maps of a step whose entry ``r`` is the request in row ``slots[r]`` of ``tables``, with ``counts[r]`` new tokens and
     ``kv_len[r]`` tokens once the step has run (int32, on the device); ``num_tokens``: the sum of the counts.  The block table is
     ``width`` columns wide (``None``: as wide as ``tables``); cells behind an entry's last page are -1, whatever ``tables`` holds
-    there.  An entry of length 0 (a row that pads the batch) has an empty row, its tokens position 0 and no slot.
+    there.  An entry of length 0 (a row that pads the batch) has an empty row; its tokens have positions from 0 on and no slot.
 
     ``out``: tensors to write into, which may have room for more entries and tokens than there are (those are left as they are);
     what is ``None`` there is not made."""

@@ -3,8 +3,13 @@ per head size.
 
 ``page_bounds`` keeps, beside the pages of keys, the least and the greatest value of every channel on each full page;
 ``choose_pages`` ranks the pages a query row sees by an upper bound of its scores on them; ``paged_attention_chosen`` attends
-to the keys of the pages chosen.  What a row chooses, and what it gets, depends on its position and the cache alone, not on
-the batch or on where a prompt was cut.
+to the keys of the pages chosen.
+
+What a row chooses depends on its query, its position and the cache, not on the batch or on where a prompt was cut, as far as
+64-bit sums go: rows of prompts and single tokens have their scores added up in different orders, so a score that lies within the
+rounding of those sums of a midpoint between two 32-bit numbers may come out one step apart.  What float32 attention makes of a choice
+does not depend on the batch; in bfloat16 the number of rows decides how a list is cut and so the order of its sums (within the
+rounding of the output).
 """
 
 from __future__ import annotations
@@ -117,7 +122,7 @@ def page_bounds(keys: torch.Tensor, bounds: torch.Tensor, *, block_table: torch.
 def choose_shape(rows: int, entries: int, kv_heads: int, width: int, head_dim: int) -> tuple[bool, int]:
     """(tiles of eight rows or not, CTAs of a cluster) of a choice.  Tiles where entries have several rows each, in clusters where the
     scores of many pages want the shared memory or few tiles would not fill the GPU.  For single tokens as many CTAs as let two a
-    multiprocessor be there at once, three where each would still have 512 pages (bfloat16, 32 heads over 8 of 128, clusters of 1, 2, 4
+    multiprocessor be there at once, three where each would still have 512 pages (bfloat16, 32 heads over 8 of 128, bounds in L2, clusters of 1, 2, 4
     and 8; 2,048 pages: 1 request 34.5, 21.5, 14.6 and 11.0 us, 8 requests 34.8, 21.9, 17.0 and 22.4, 24 requests 51.6, 41.4, 44.9 and
     59.0, 64 requests 79, 91, 109 and 145; 512 pages: 1 request 12.4, 9.5, 7.8 and 6.7, 24 requests 14.3, 18.5, 21.7 and 33.3)."""
 
