@@ -290,13 +290,16 @@ def test_no_static_is_shared_by_libraries_that_configure_kernels_of_their_own():
     the libraries that are built)."""
 
     import collections
-    import pathlib
     import shutil
     import subprocess
 
     from llm_runtime_study_b200.csrc import build
 
-    built = sorted(pathlib.Path(build.CSRC_DIR, "_build").glob("lib*.so"))
+    for head_dim in range(16, 257, 16):
+        sparse_pages.library_name(head_dim)
+    specs = native.library_specs()
+    paths = [build.library_path(name, sources, native.library_defines(name))[0] for name, sources in specs.items()]
+    built = [path for path in paths if path.is_file()]
     if not built or shutil.which("nm") is None:
         pytest.skip("no libraries are built here")
     shared = collections.Counter()
